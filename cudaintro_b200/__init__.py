@@ -12,9 +12,9 @@ The binding (:mod:`cudaintro_b200.capi`) is imported on first attribute access, 
 import importlib
 
 _CAPI_NAMES = (
-    "B200Error", "COL_MAJOR_NN", "F32_3XTF32", "F32_FFMA", "F32_TF32", "ROW_MAJOR", "ROW_MAJOR_BT", "check_device", "fill",
-    "gemm_16_f32", "gemm_bf16", "gemm_f16", "gemm_f32", "gemm_host", "gemm_i8_i32", "gemm_naive", "gemm_w8a8_bf16", "lib", "linear",
-    "quantize_absmax", "set_tile_policy", "time_gemm",
+    "B200Error", "COL_MAJOR_NN", "F32_3XTF32", "F32_FFMA", "F32_TF32", "ROW_MAJOR", "ROW_MAJOR_BT", "check_device",
+    "dequantize_mxfp4", "fill", "gemm_16_f32", "gemm_bf16", "gemm_f16", "gemm_f32", "gemm_host", "gemm_i8_i32", "gemm_mxfp4",
+    "gemm_naive", "gemm_w8a8_bf16", "lib", "linear", "linear_mxfp4", "quantize_absmax", "quantize_mxfp4", "set_tile_policy", "time_gemm",
 )
 
 

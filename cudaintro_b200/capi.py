@@ -40,6 +40,13 @@ SIGNATURES = {
     "b200_fill_f32": (_int, [_p, _i64, C.c_uint64, C.c_float, C.c_float, _p]),
     "b200_gemm_naive": (_int, [_int, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p]),
     "b200_linear": (_int, [_int, _p, _p, _p, _p, _i64, _i64, _i64, _int, _int, _int, _p]),
+    "b200_mxfp4_row_bytes": (C.c_size_t, [_i64]),
+    "b200_mxfp4_scale_bytes": (C.c_size_t, [_i64, _i64]),
+    "b200_quantize_mxfp4": (_int, [_int, _p, _p, _p, _i64, _i64, _i64, _int, _p]),
+    "b200_dequantize_mxfp4": (_int, [_int, _p, _p, _p, _i64, _i64, _i64, _p]),
+    "b200_gemm_mxfp4": (_int, [_int, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p]),
+    "b200_linear_mxfp4_workspace": (C.c_size_t, [_i64, _i64]),
+    "b200_linear_mxfp4": (_int, [_int, _p, _p, _p, _p, _p, _i64, _i64, _i64, _int, _p, C.c_size_t, _p]),
     "b200_gemm_host": (_int, [_int, _p, _p, _p, _i64, _i64, _i64, _int]),
     "b200_host_release": (_int, []),
     "b200_host_weights_upload": (_int, [_int, _p, _i64, _i64, C.POINTER(C.c_void_p)]),
@@ -227,6 +234,126 @@ def linear(x, w, bias=None, w_layout=ROW_MAJOR_BT, relu=False, bias_first=False,
     with torch.cuda.device(x.device):
         _check(lib.b200_linear(_code(x.dtype), x.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(),
                                out.data_ptr(), batch, in_f, out_f, w_layout, flags, mode, _stream()))
+    return out
+
+
+# ------------------------------------------------------------------ 4-bit (MXFP4)
+
+def _launch(device, fn, *args) -> None:
+    """One call of the library on the current stream of `device`."""
+    import torch
+
+    if device.index == torch.cuda.current_device():
+        _check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            _check(fn(*args, torch.cuda.current_stream().cuda_stream))
+
+
+def _require(ok: bool, message: str) -> None:
+    if not ok:
+        raise ValueError(message)
+
+
+def _mx_operand(name, q, scale, device=None):
+    """(rows, K in whole blocks) of a packed matrix whose two tensors belong together."""
+    import torch
+
+    _require(q.dtype == torch.uint8 and q.dim() == 2 and q.is_cuda and q.is_contiguous() and q.shape[0] > 0
+             and q.shape[1] > 0 and q.shape[1] % 16 == 0,
+             f"{name}: packed elements are a contiguous uint8 CUDA tensor [rows, whole blocks of 16 bytes]")
+    rows, width = q.shape
+    _require(scale.dtype == torch.uint8 and scale.is_contiguous()
+             and tuple(scale.shape) == (-(-rows // 128), -(-width // 64), 32, 4, 4) and scale.device == q.device,
+             f"{name}: scales are a contiguous uint8 tensor [{-(-rows // 128)}, {-(-width // 64)}, 32, 4, 4] beside them")
+    _require(device is None or q.device == device, f"{name}: operands are on different devices")
+    return rows, 2 * width
+
+
+def _mx_out(out, shape, dtype, device):
+    import torch
+
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _require(out.dtype == dtype and tuple(out.shape) == shape and out.device == device and out.is_contiguous(),
+             f"out: a contiguous {dtype} tensor {list(shape)} on {device}")
+    return out
+
+
+def quantize_mxfp4(x, along: int = 0):
+    """x: [R, C] fp32, fp16 or bf16 CUDA tensor (rows may be strided) -> (q, scale) with blocks of 32 along the
+    rows (along = 0: q is uint8 [R, 16 * ceil(C / 32)]) or down the columns (along = 1: the result is
+    transposed, q is uint8 [C, 16 * ceil(R / 32)]).  scale: uint8 [bands of 128 rows, tiles of 4 blocks, 32, 4, 4],
+    the byte of (row, block) at [row // 128, block // 4, row % 32, row % 128 // 32, block % 4]."""
+    import torch
+
+    _require(x.dim() == 2 and x.is_cuda and x.dtype in (torch.float32, torch.float16, torch.bfloat16),
+             "x: a 2-D fp32, fp16 or bf16 CUDA tensor")
+    R, Cc = x.shape
+    _require(R > 0 and Cc > 0, "x: sizes must be positive")
+    _require(Cc == 1 or x.stride(1) == 1, "x: elements of a row must be neighbours")
+    _require(along in (0, 1), "along: 0 (blocks in rows) or 1 (blocks in columns)")
+    ldx = x.stride(0) if R > 1 else Cc
+    _require(ldx >= Cc, "x: rows must not overlap")
+    rows, K = (Cc, R) if along else (R, Cc)
+    q = torch.empty((rows, -(-K // 32) * 16), dtype=torch.uint8, device=x.device)
+    scale = torch.empty((-(-rows // 128), -(-K // 128), 32, 4, 4), dtype=torch.uint8, device=x.device)
+    _launch(x.device, lib.b200_quantize_mxfp4, _code(x.dtype), x.data_ptr(), q.data_ptr(), scale.data_ptr(), R, Cc, ldx,
+            along)
+    return q, scale
+
+
+def dequantize_mxfp4(q, scale, K=None, dtype=None, out=None):
+    """(q, scale) -> [rows, K] values in `dtype` (bf16 if not given).  K: the row length that was quantised (whole
+    blocks if not given)."""
+    import torch
+
+    rows, width = _mx_operand("q", q, scale)
+    K = width if K is None else K
+    _require(width - 32 < K <= width, f"K: between {width - 31} and {width} for rows of {q.shape[1]} bytes")
+    dtype = torch.bfloat16 if dtype is None else dtype
+    _require(dtype in (torch.float32, torch.float16, torch.bfloat16), "dtype: fp32, fp16 or bf16")
+    out = _mx_out(out, (rows, K), dtype, q.device)
+    _launch(q.device, lib.b200_dequantize_mxfp4, _code(dtype), q.data_ptr(), scale.data_ptr(), out.data_ptr(), rows, K, 0)
+    return out
+
+
+def gemm_mxfp4(a, a_scale, b, b_scale, dtype=None, out=None):
+    """a [M, K] times b [N, K] transposed, both packed 4-bit, fp32 sums, result in `dtype` (bf16 if not given)."""
+    import torch
+
+    M, K = _mx_operand("a", a, a_scale)
+    N, K2 = _mx_operand("b", b, b_scale, a.device)
+    if K != K2:
+        raise ValueError(f"inner dimensions differ: {K} vs {K2}")
+    dtype = torch.bfloat16 if dtype is None else dtype
+    _require(dtype in (torch.float32, torch.float16, torch.bfloat16), "dtype: fp32, fp16 or bf16")
+    out = _mx_out(out, (M, N), dtype, a.device)
+    _launch(a.device, lib.b200_gemm_mxfp4, _code(dtype), a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
+            b_scale.data_ptr(), out.data_ptr(), M, N, K, 0)
+    return out
+
+
+def linear_mxfp4(x, w, w_scale, bias=None, relu=False, out=None):
+    """Fully connected layer on 4-bit weights: act(Q(x) @ W^T + bias), x [batch, in] fp32, fp16 or bf16 quantised along
+    its rows on the way, (w, w_scale) the quantised [out, in] weights, bias fp32 [out]."""
+    import torch
+
+    _require(x.dim() == 2 and x.is_cuda and x.is_contiguous() and x.shape[0] > 0
+             and x.dtype in (torch.float32, torch.float16, torch.bfloat16),
+             "x: a contiguous 2-D fp32, fp16 or bf16 CUDA tensor")
+    batch, in_f = x.shape
+    out_f, K = _mx_operand("w", w, w_scale, x.device)
+    _require(K - 32 < in_f <= K, f"inner dimensions differ: {in_f} vs {K}")
+    if bias is not None:
+        _require(bias.dtype == torch.float32 and tuple(bias.shape) == (out_f,) and bias.is_contiguous()
+                 and bias.device == x.device, f"bias: a contiguous fp32 tensor [{out_f}] on {x.device}")
+    out = _mx_out(out, (batch, out_f), x.dtype, x.device)
+    need = batch * (K // 2) + -(-batch // 128) * -(-K // 128) * 512
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _launch(x.device, lib.b200_linear_mxfp4, _code(x.dtype), x.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
+            0 if bias is None else bias.data_ptr(), out.data_ptr(), batch, in_f, out_f, LINEAR_RELU if relu else 0,
+            ws.data_ptr(), need)
     return out
 
 

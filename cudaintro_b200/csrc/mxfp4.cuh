@@ -1,0 +1,81 @@
+// The MXFP4 format on the device: scale bytes, element codes, and where a scale byte lies.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "internal.h"
+
+namespace b200 {
+
+// A product of two 4-bit matrices, C[M,N] = A[M,K] * B[N,K]^T, with the optional tail of a layer.
+struct MxGemm {
+  const uint8_t* A = nullptr;
+  const uint8_t* a_scale = nullptr;
+  const uint8_t* B = nullptr;
+  const uint8_t* b_scale = nullptr;
+  void* C = nullptr;
+  int64_t M = 0, N = 0, K = 0, ldc = 0;
+  Tail tail;
+};
+
+// Bytes of one packed row: whole blocks of 32 elements, 16 bytes each.
+__host__ __device__ __forceinline__ int64_t mx_row_bytes(int64_t K) { return (K + 31) / 32 * 16; }
+
+// Scale bytes lie in tiles of 128 rows x 4 blocks (512 bytes; `words` tiles along K make a band): in a
+// tile, 32 lines of 16 bytes, line l holding the four bytes of rows l, l + 32, l + 64, l + 96.  One
+// tcgen05.cp.32x128b moves such a tile into four columns of tensor memory, where the tensor cores
+// look for it.
+__host__ __device__ __forceinline__ int64_t mx_scale_offset(int64_t row, int64_t block, int64_t words) {
+  return ((row >> 7) * words + (block >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
+}
+
+// |v| as an integer that orders like the magnitude, with NaN above infinity: a maximum over a block
+// keeps what is not finite in sight.
+__device__ __forceinline__ uint32_t mx_magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// Scale byte of a block whose largest magnitude has the bits `top`: the element format's largest power
+// of two is 4, so the exponent is floor(log2 max) - 2, kept at -127 and above (zero blocks too).  A block
+// with an infinity or a NaN in it gets 255, the scale format's NaN.
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t top) {
+  const uint32_t e = top >> 23;
+  return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+}
+
+// Codes of eight elements under a scale byte, element i in bits [4i, 4i + 4): x / 2^E rounded to nearest,
+// ties to the even code, magnitudes beyond 6 taken to 6.  1 / 2^E is a normal fp32 number for every
+// byte up to 253, so the product is exact wherever it does not vanish.
+__device__ __forceinline__ uint32_t mx_encode8(const float (&v)[8], uint32_t byte) {
+  if (byte == 255u) return 0u;
+  const float inv = __uint_as_float((254u - byte) << 23);
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t pair;
+    asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\tcvt.u32.u8 %0, b;\n\t}"
+        : "=r"(pair)
+        : "f"(v[2 * i + 1] * inv), "f"(v[2 * i] * inv));
+    r |= pair << (8 * i);
+  }
+  return r;
+}
+
+// Value of a scale byte: 2^(byte - 127); 0 is a subnormal fp32 number, 255 is NaN.
+__device__ __forceinline__ float mx_scale_value(uint32_t byte) {
+  return byte == 255u ? __uint_as_float(0x7fffffffu) : byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
+}
+
+// Values of eight codes, times the scale.
+__device__ __forceinline__ void mx_decode8(uint32_t codes, uint32_t byte, float (&v)[8]) {
+  const float s = mx_scale_value(byte);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t h;
+    asm("{\n\t.reg .b8 b;\n\tcvt.u8.u32 b, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(h) : "r"(codes >> (8 * i)));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    v[2 * i] = f.x * s;
+    v[2 * i + 1] = f.y * s;
+  }
+}
+
+}  // namespace b200

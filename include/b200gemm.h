@@ -275,6 +275,55 @@ typedef enum b200_linear_flags { B200_LINEAR_RELU = 1, B200_LINEAR_BIAS_FIRST = 
 int b200_linear(int dtype, const void* X, const void* W, const float* bias, void* Y, int64_t batch,
                 int64_t in_features, int64_t out_features, int w_layout, int flags, int f32_mode, void* stream);
 
+/* Microscaled 4-bit floating point, MXFP4 (Open Compute Project, microscaling formats 1.0): 32
+ * neighbours along K share a scale byte s, the power of two 2^(s - 127) (255 = NaN); an element is 4 bits,
+ * sign, two of exponent, one of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6.  No counterpart in the reference,
+ * whose quantised path stops at 8 bits (quantization/GEMM_int8.cu:21-91).
+ *   packed elements  [rows][b200_mxfp4_row_bytes(K)] bytes, K contiguous, two elements a byte with the even
+ *                    one in the low half; a row is whole blocks (16 bytes each), and the elements that fill
+ *                    up the last one are zero.
+ *   scales           b200_mxfp4_scale_bytes(rows, K) bytes in tiles of 128 rows x 4 blocks: with T =
+ *                    ceil(K / 128), the byte of row r and block b is at
+ *                      ((r / 128) * T + b / 4) * 512 + (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4.
+ *                    Bytes of rows and blocks that only fill up a tile must not be 255 (the quantiser
+ *                    writes 0).
+ * Both arrays are 16-byte aligned, else B200_ERR_UNSUPPORTED. */
+size_t b200_mxfp4_row_bytes(int64_t K);
+size_t b200_mxfp4_scale_bytes(int64_t rows, int64_t K);
+
+/* Quantises a row-major [R, C] matrix of B200_F32, B200_F16 or B200_BF16 (leading dimension ldx, 0 = C).
+ *   along = 0: blocks run along the rows; the result has R rows of K = C elements;
+ *   along = 1: blocks run down the columns and the result is stored transposed, C rows of K = R elements:
+ *              weights kept [in, out] become the [out, in] form the products take, and the two gradient
+ *              products of a layer, which sum over rows, get their operands.
+ * Per block: exponent floor(log2(max |x|)) - 2 (at least -127), elements x / 2^exponent to nearest, ties to
+ * the even code, magnitudes above 6 taken to 6.  An infinity or NaN makes its whole block NaN (scale
+ * 255, elements 0); a block of zeros has scale 0.  x has no alignment rule beyond its element size. */
+int b200_quantize_mxfp4(int dtype, const void* x, void* q, void* scale, int64_t R, int64_t C, int64_t ldx, int along,
+                        void* stream);
+
+/* The way back: x[r][k] = element * 2^(s - 127), rounded once to `dtype`; x [rows, K] with leading dimension
+ * ldx (0 = K).  Nothing beyond column K of a row is written. */
+int b200_dequantize_mxfp4(int dtype, const void* q, const void* scale, void* x, int64_t rows, int64_t K, int64_t ldx,
+                          void* stream);
+
+/* C[m][n] = sum_k A[m][k] * B[n][k] of two packed matrices (both K contiguous, B stored [N, K]) on the tensor
+ * cores: exact products, fp32 sums, rounded once to out_dtype (B200_F32, B200_F16, B200_BF16).  A NaN block
+ * makes the outputs that take it NaN.  ldc = 0 means N; C has no alignment rule beyond its element size. */
+int b200_gemm_mxfp4(int out_dtype, const void* A, const void* a_scale, const void* B, const void* b_scale, void* C,
+                    int64_t M, int64_t N, int64_t K, int64_t ldc, void* stream);
+
+/* Fully connected layer on 4-bit weights: Y = act(Q(X) W^T + bias), where Q is b200_quantize_mxfp4 along the
+ * rows.  X [batch, in_features] and Y [batch, out_features] are packed row-major matrices of `dtype` (B200_F32,
+ * B200_F16 or B200_BF16); W and w_scale a quantised [out_features, in_features] matrix; bias and flags as in
+ * b200_linear (the bias is added to the finished fp32 sum).  workspace: device memory for the quantised X,
+ * 16-byte aligned, at least b200_linear_mxfp4_workspace(batch, in_features) bytes; a call uses it until its
+ * work on `stream` is done, so calls that may overlap need one each. */
+size_t b200_linear_mxfp4_workspace(int64_t batch, int64_t in_features);
+int b200_linear_mxfp4(int dtype, const void* X, const void* W, const void* w_scale, const float* bias, void* Y,
+                      int64_t batch, int64_t in_features, int64_t out_features, int flags, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 /* Same products with HOST buffers: copies A and B to the device, runs the kernels, copies C
  * back, and returns after the result is in `C`.  `dtype` selects the entry point above
  * (B200_I8 -> int32 out, B200_F16 / B200_BF16 -> 16-bit out, B200_F32 -> FFMA).  The operand
