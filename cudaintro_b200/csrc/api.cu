@@ -250,6 +250,9 @@ extern "C" int b200_check_device(void* stream) {
   rc = read_and_clear_skinny_status(&st_skinny);
   if (rc) return rc;
   st |= st_skinny << 8;
+  rc = read_and_clear_mx_status(&st_skinny);
+  if (rc) return rc;
+  st |= st_skinny << 16;
   if (st) return fail(B200_ERR_DEVICE_WAIT, "a tensor-core kernel gave up a bounded wait (status 0x%x)", st);
   return B200_OK;
 }

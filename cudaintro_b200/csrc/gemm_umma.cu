@@ -1079,7 +1079,31 @@ int encode_operand_map(CUtensorMap* map, int kind, const void* base, int64_t row
   return make_map(map, kind, base, rows, cols, ld, box_cols, box_rows, chunks32);
 }
 
+int encode_tiled_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
+                     const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle,
+                     CUtensorMapL2promotion promotion) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t d[5], st[5];
+  cuuint32_t b[5], estr[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    estr[i] = 1;
+    if (i + 1 < rank) st[i] = strides[i];
+  }
+  CUresult r = enc(map, type, cuuint32_t(rank), const_cast<void*>(base), d, st, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   swizzle, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", int(r));
+  return B200_OK;
+}
+
 bool dependent_launch_enabled() { return g_use_pdl; }
+
+void wait_test_settings(int* lose_kb, unsigned long long* budget_ns) {
+  *lose_kb = g_lose_kb;
+  *budget_ns = g_wait_budget_ns;
+}
 
 int set_tile_policy(int cg, int bn, int group_rows) {
   if (group_rows < 0 || (group_rows % 256) != 0)

@@ -65,6 +65,19 @@ int read_and_clear_skinny_status(uint32_t* out);
 int encode_operand_map(CUtensorMap* map, int kind, const void* base, int64_t rows, int64_t cols, int64_t ld,
                        int box_cols, int box_rows, bool chunks32);
 
+// Any tiled tensor map: `rank` dimensions (innermost first), strides in bytes of dimensions 1.., zero fill.
+int encode_tiled_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
+                     const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle,
+                     CUtensorMapL2promotion promotion);
+
+// Product of two 4-bit matrices (gemm_mxfp4.cu); out_dtype is B200_F32, B200_F16 or B200_BF16.
+struct MxGemm;
+int launch_mx_gemm(int out_dtype, const MxGemm& g, cudaStream_t stream);
+int read_and_clear_mx_status(uint32_t* out);
+
+// What set_wait_test left: the k-block to lose (-1 = none) and the limit of a single wait.
+void wait_test_settings(int* lose_kb, unsigned long long* budget_ns);
+
 // Whether kernels are launched with programmatic stream serialisation (set_dependent_launch).
 bool dependent_launch_enabled();
 

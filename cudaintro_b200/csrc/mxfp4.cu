@@ -150,49 +150,6 @@ mx_dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ 
   }
 }
 
-// Product on the CUDA cores: a 64 x 64 tile of C, one block of K at a time decoded into shared memory.
-template <typename T>
-__global__ void __launch_bounds__(256)
-mx_gemm_simt_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ sa, const uint8_t* __restrict__ B,
-                    const uint8_t* __restrict__ sb, T* __restrict__ C, int64_t M, int64_t N, int64_t K, int64_t ldc,
-                    const float* __restrict__ bias, int relu) {
-  __shared__ float ta[32][65], tb[32][65];
-  const int64_t row_bytes = mx_row_bytes(K), blocks = row_bytes / 16, words = (blocks + 3) / 4;
-  const int64_t m0 = int64_t(blockIdx.y) * 64, n0 = int64_t(blockIdx.x) * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int lr = threadIdx.x >> 2, lk = (threadIdx.x & 3) * 8;  // the row and the eight elements this thread decodes
-  float acc[4][4] = {};
-  for (int64_t kb = 0; kb < blocks; ++kb) {
-    float v[8];
-    const int64_t at = kb * 16 + (lk >> 1);
-    mx_decode8(m0 + lr < M ? *reinterpret_cast<const uint32_t*>(A + (m0 + lr) * row_bytes + at) : 0u,
-               m0 + lr < M ? sa[mx_scale_offset(m0 + lr, kb, words)] : 0, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ta[lk + i][lr] = v[i];
-    mx_decode8(n0 + lr < N ? *reinterpret_cast<const uint32_t*>(B + (n0 + lr) * row_bytes + at) : 0u,
-               n0 + lr < N ? sb[mx_scale_offset(n0 + lr, kb, words)] : 0, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) tb[lk + i][lr] = v[i];
-    __syncthreads();
-    for (int k = 0; k < 32; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(ta[k][ty + 16 * i], tb[k][tx + 16 * j], acc[i][j]);
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m < M && n < N) {
-        float y = acc[i][j] + (bias ? bias[n] : 0.0f);
-        C[m * ldc + n] = from_f32<T>(relu ? fmaxf(0.0f, y) : y);
-      }
-    }
-}
-
 template <typename T>
 int quantize_t(const T* x, uint8_t* q, uint8_t* scale, int64_t R, int64_t C, int64_t ldx, int along, cudaStream_t stream) {
   if (along == 0) {
@@ -219,16 +176,6 @@ int dequantize_t(const uint8_t* q, const uint8_t* scale, T* x, int64_t rows, int
   const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * int64_t(sizeof(T)) % 16 == 0;
   if (vec) mx_dequantize_kernel<T, true><<<grid, kMxThreads, 0, stream>>>(q, scale, x, rows, K, ldx, words, units);
   else mx_dequantize_kernel<T, false><<<grid, kMxThreads, 0, stream>>>(q, scale, x, rows, K, ldx, words, units);
-  B200_CUDA_TRY(cudaGetLastError());
-  return B200_OK;
-}
-
-template <typename T>
-int gemm_t(const MxGemm& g, cudaStream_t stream) {
-  dim3 grid(unsigned((g.N + 63) / 64), unsigned((g.M + 63) / 64));
-  if (grid.y > 65535) return fail(B200_ERR_TOO_LARGE, "MXFP4 product: more than %lld rows", 65535LL * 64);
-  mx_gemm_simt_kernel<T><<<grid, 256, 0, stream>>>(g.A, g.a_scale, g.B, g.b_scale, static_cast<T*>(g.C), g.M, g.N, g.K,
-                                                   g.ldc, g.tail.bias, g.tail.flags & B200_LINEAR_RELU);
   B200_CUDA_TRY(cudaGetLastError());
   return B200_OK;
 }
@@ -262,14 +209,6 @@ int quantize(int dtype, const void* x, void* q, void* scale, int64_t R, int64_t 
     case B200_F32: return quantize_t(static_cast<const float*>(x), q8, s8, R, C, ldx, along, stream);
     case B200_F16: return quantize_t(static_cast<const __half*>(x), q8, s8, R, C, ldx, along, stream);
     default: return quantize_t(static_cast<const __nv_bfloat16*>(x), q8, s8, R, C, ldx, along, stream);
-  }
-}
-
-int gemm(int out_dtype, const MxGemm& g, cudaStream_t stream) {
-  switch (out_dtype) {
-    case B200_F32: return gemm_t<float>(g, stream);
-    case B200_F16: return gemm_t<__half>(g, stream);
-    default: return gemm_t<__nv_bfloat16>(g, stream);
   }
 }
 
@@ -330,7 +269,7 @@ extern "C" int b200_gemm_mxfp4(int out_dtype, const void* A, const void* a_scale
   g.N = N;
   g.K = K;
   g.ldc = ldc;
-  return gemm(out_dtype, g, static_cast<cudaStream_t>(stream));
+  return launch_mx_gemm(out_dtype, g, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t b200_linear_mxfp4_workspace(int64_t batch, int64_t in_features) {
@@ -370,5 +309,5 @@ extern "C" int b200_linear_mxfp4(int dtype, const void* X, const void* W, const 
   g.ldc = out_features;
   g.tail.bias = bias;
   g.tail.flags = flags;
-  return gemm(dtype, g, stream);
+  return launch_mx_gemm(dtype, g, stream);
 }
