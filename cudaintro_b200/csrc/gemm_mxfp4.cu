@@ -50,6 +50,23 @@ __host__ __device__ constexpr uint32_t mx_instr_desc(int mma_m, int mma_n, int s
          (uint32_t(mma_m >> 4) << 24) | (uint32_t(scale_id) << 29);
 }
 
+// One lane of a converged warp.  The TMA, copy and MMA loops below are run by whole warps that elect a lane around
+// the asynchronous instructions themselves: the compiler then keeps descriptors and addresses in uniform registers.
+// With the loops inside a branch on lane 0 every tcgen05.cp cost the issuing lane 45 clocks and every MMA 45 to 60
+// (six copies and four MMAs 800 clocks against the 512 that the MMAs run); elected, six copies cost 50 together.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e != 0;
+}
+
+// A bounded wait of a whole warp, with one outcome for all its lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint64_t budget_ns) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, budget_ns)) != 0;
+}
+
 template <int CG>
 __device__ __forceinline__ void mx_umma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa_tmem,
                                         uint32_t sb_tmem, uint32_t accumulate) {
@@ -227,21 +244,18 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      int stage = 0, it = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int t = first_tile; t < num_tiles && ok; t += tile_step, ++it) {
-        int mb, nb;
-        mx_tile_coords(t, p, mb, nb);
-        const int m0 = mb * T::TILE_M + int(cta_rank) * 128;
-        const int n0 = nb * BN + int(cta_rank) * (BN / CG);
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_budget_ns)) { ok = false; break; }
-          if (kb == p.lose_kb && it == 0 && blockIdx.x == 0) {
-            if (++stage == T::STAGES) { stage = 0; phase ^= 1u; }
-            continue;
-          }
+    int stage = 0, it = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int t = first_tile; t < num_tiles && ok; t += tile_step, ++it) {
+      int mb, nb;
+      mx_tile_coords(t, p, mb, nb);
+      const int m0 = mb * T::TILE_M + int(cta_rank) * 128;
+      const int n0 = nb * BN + int(cta_rank) * (BN / CG);
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (!warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_budget_ns)) { ok = false; break; }
+        const bool lost = kb == p.lose_kb && it == 0 && blockIdx.x == 0;
+        if (!lost && elect_lane()) {
           uint8_t* sa = smem + stage * T::STAGE_BYTES;
           uint8_t* sb = sa + T::A_BYTES;
           uint8_t* ssa = sb + T::B_BYTES;
@@ -260,21 +274,22 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             mx_load_3d<CG>(ssa, &tmap_sa, smem_u32(&full_bar[stage]), 0, kb * 2, m0 >> 7);
             mx_load_3d<CG>(ssb, &tmap_sb, smem_u32(&full_bar[stage]), 0, kb * 2, nb * T::BANDS);
           }
-          if (++stage == T::STAGES) { stage = 0; phase ^= 1u; }
         }
+        __syncwarp();
+        if (++stage == T::STAGES) { stage = 0; phase ^= 1u; }
       }
-      if constexpr (CG == 2) {
-        // Stay until every stage has been released: the releases are arrivals of the leader's commits in this
-        // CTA's shared memory, which must still exist.
-        for (int i = 0; i < T::STAGES && ok; ++i) {
-          ok = mbar_wait_bounded(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_budget_ns);
-          if (++stage == T::STAGES) { stage = 0; phase ^= 1u; }
-        }
+    }
+    if constexpr (CG == 2) {
+      // Stay until every stage has been released: the releases are arrivals of the leader's commits in this
+      // CTA's shared memory, which must still exist.
+      for (int i = 0; i < T::STAGES && ok; ++i) {
+        ok = warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_budget_ns);
+        if (++stage == T::STAGES) { stage = 0; phase ^= 1u; }
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ scale copies and MMAs
-    if (lane == 0 && cta_rank == 0) {
+    if (cta_rank == 0) {
       constexpr uint32_t idesc0 = mx_instr_desc(T::TILE_M, BN, 0), idesc2 = mx_instr_desc(T::TILE_M, BN, 2);
       const uint32_t ring = smem_u32(smem);
       const uint64_t a_desc0 = make_smem_desc_sw128(ring, 16, 1024);
@@ -289,41 +304,44 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       for (int t = first_tile; t < num_tiles && ok; t += tile_step, ++it) {
         const int ab = it & 1;
         // the epilogue is done with the tile before the last, and with what the last one shares with this one
-        if (!mbar_wait_bounded(acc_go, uint32_t(it + 1) & 1u, abort_flag, p.wait_budget_ns)) break;
-        tc_fence_after_sync();
+        if (!warp_wait(acc_go, uint32_t(it + 1) & 1u, abort_flag, p.wait_budget_ns)) break;
         const uint32_t d_tmem = tmem_base + uint32_t(ab * T::ACC_STEP);
         for (int kb = 0; kb < num_kb; ++kb, ++count) {
-          if (!mbar_wait_bounded(&full_bar[stage], phase, abort_flag, p.wait_budget_ns)) { ok = false; break; }
+          if (!warp_wait(&full_bar[stage], phase, abort_flag, p.wait_budget_ns)) { ok = false; break; }
           if (count >= 2) {
-            if (!mbar_wait_bounded(&empty_bar[behind], behind_phase, abort_flag, p.wait_budget_ns)) { ok = false; break; }
+            if (!warp_wait(&empty_bar[behind], behind_phase, abort_flag, p.wait_budget_ns)) { ok = false; break; }
             if (++behind == T::STAGES) { behind = 0; behind_phase ^= 1u; }
           }
           tc_fence_after_sync();
           const uint32_t sa_tmem = tmem_base + uint32_t(T::SCALE_COL) + (count & 1u) * uint32_t(T::SCALE_STEP);
           const uint32_t sb_tmem = sa_tmem + 8;
           const uint64_t s_desc = s_desc0 + uint64_t(stage) * kStageStep;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            mx_copy_scales<CG>(sa_tmem + uint32_t(4 * h), s_desc + uint64_t((h * kScaleTile) >> 4));
-#pragma unroll
-            for (int b = 0; b < T::BANDS; ++b)
-              mx_copy_scales<CG>(sb_tmem + uint32_t(h * 4 * T::BANDS + 4 * b),
-                                 s_desc + uint64_t((T::SA_BYTES + (2 * b + h) * kScaleTile) >> 4));
-          }
           const uint64_t a_desc = a_desc0 + uint64_t(stage) * kStageStep;
           const uint64_t b_desc = b_desc0 + uint64_t(stage) * kStageStep;
           const int left = p.blocks - kb * 8;  // blocks of 32 this stage really holds
+          if (elect_lane()) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (2 * j < left)
-              mx_umma<CG>(d_tmem, a_desc + uint64_t(2 * j), b_desc + uint64_t(2 * j), (j & 1) ? idesc2 : idesc0,
-                          sa_tmem + uint32_t(4 * (j >> 1)), sb_tmem + uint32_t(4 * T::BANDS * (j >> 1)), (kb | j) != 0 ? 1u : 0u);
+            for (int h = 0; h < 2; ++h) {
+              mx_copy_scales<CG>(sa_tmem + uint32_t(4 * h), s_desc + uint64_t((h * kScaleTile) >> 4));
+#pragma unroll
+              for (int b = 0; b < T::BANDS; ++b)
+                mx_copy_scales<CG>(sb_tmem + uint32_t(h * 4 * T::BANDS + 4 * b),
+                                   s_desc + uint64_t((T::SA_BYTES + (2 * b + h) * kScaleTile) >> 4));
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (2 * j < left)
+                mx_umma<CG>(d_tmem, a_desc + uint64_t(2 * j), b_desc + uint64_t(2 * j), (j & 1) ? idesc2 : idesc0,
+                            sa_tmem + uint32_t(4 * (j >> 1)), sb_tmem + uint32_t(4 * T::BANDS * (j >> 1)),
+                            (kb | j) != 0 ? 1u : 0u);
+            }
+            if constexpr (CG == 2) umma_commit_pair(&empty_bar[stage], 3); else umma_commit(&empty_bar[stage]);
+            if (kb + 1 == num_kb) {
+              if constexpr (CG == 2) umma_commit_pair(&acc_full[ab], 3); else umma_commit(&acc_full[ab]);
+            }
           }
-          if constexpr (CG == 2) umma_commit_pair(&empty_bar[stage], 3); else umma_commit(&empty_bar[stage]);
+          __syncwarp();
           if (++stage == T::STAGES) { stage = 0; phase ^= 1u; }
-        }
-        if (ok) {
-          if constexpr (CG == 2) umma_commit_pair(&acc_full[ab], 3); else umma_commit(&acc_full[ab]);
         }
       }
     }
