@@ -20,5 +20,7 @@ _CAPI_NAMES = (
 
 def __getattr__(name):
     if name in _CAPI_NAMES:
-        return getattr(importlib.import_module(".capi", __name__), name)
+        # kept, so that only the first access of a name comes here (an access cost more than a microsecond)
+        globals()[name] = value = getattr(importlib.import_module(".capi", __name__), name)
+        return value
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
