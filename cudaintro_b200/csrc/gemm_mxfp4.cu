@@ -163,7 +163,7 @@ __device__ __forceinline__ void mx_finish(const MxArgs& p, int n0, uint32_t (&v)
   if (p.bias != nullptr) {
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-      v[i] = __float_as_uint(__uint_as_float(v[i]) + __ldg(p.bias + min(n0 + i, p.N - 1)));
+      v[i] = __float_as_uint(__uint_as_float(v[i]) + p.bias[min(n0 + i, p.N - 1)]);
   }
   if (p.relu) {
 #pragma unroll

@@ -16,168 +16,310 @@ namespace {
 constexpr int kMxThreads = 256;
 
 template <typename T>
-__device__ __forceinline__ float to_f32(T v) {
-  if constexpr (std::is_same<T, float>::value) return v;
-  else if constexpr (std::is_same<T, __half>::value) return __half2float(v);
-  else return __bfloat162float(v);
-}
-template <typename T>
 __device__ __forceinline__ T from_f32(float v) {
   if constexpr (std::is_same<T, float>::value) return v;
   else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
   else return __float2bfloat16_rn(v);
 }
 
-// Eight neighbours of a row as fp32; elements at or beyond `left` (how many the row still has) are 0.
-// VEC: the address is 16-byte aligned.
+// Set-up of a kernel in a stream: wait for the one before it, and let the next one (the product that takes what is
+// quantised here) begin its own.  Nothing these kernels read is declared read-only for their lifetime (no __ldg, no
+// __restrict__): the compiler may move such loads up past this wait.
+__device__ __forceinline__ void mx_follow_stream() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Sixteen neighbours of a row, as they lie in memory: words of two 16-bit values, or of one fp32 value.
+template <typename T>
+struct Sixteen {
+  static constexpr int WORDS = 4 * sizeof(T);
+  uint32_t w[WORDS];
+};
+// Elements at or beyond `left` (how many the row still has) are 0.  VEC: the address is 16-byte aligned.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* __restrict__ src, int64_t left, float (&v)[8]) {
-  if (VEC && left >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(src));
-      const T* e = reinterpret_cast<const T*>(&a);
+__device__ __forceinline__ void load16(const T* src, int64_t left, Sixteen<T>& v) {
+  if (VEC && left >= 16) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+    for (int i = 0; i < Sixteen<T>::WORDS / 4; ++i) {
+      const uint4 u = __ldcg(reinterpret_cast<const uint4*>(src) + i);
+      v.w[4 * i] = u.x; v.w[4 * i + 1] = u.y; v.w[4 * i + 2] = u.z; v.w[4 * i + 3] = u.w;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < left ? to_f32(src[i]) : 0.0f;
+    for (int i = 0; i < 16; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        v.w[i] = i < left ? __float_as_uint(src[i]) : 0u;
+      } else {
+        const uint32_t e = i < left ? reinterpret_cast<const uint16_t*>(src)[i] : 0u;
+        v.w[i / 2] = i & 1 ? v.w[i / 2] | (e << 16) : e;
+      }
+    }
   }
 }
 
-// Blocks along the rows of x [R, C].  Sixteen lanes take one word of four scales (128 elements of a
-// row), eight elements a lane: a block's largest magnitude is a maximum over four lanes, its code
-// words leave as 64 contiguous bytes, its four scale bytes as one word.  The grid also covers the
-// rows that pad the last band of 128, whose scale bytes are zero.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kMxThreads)
-mx_quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ scale, int64_t R,
-                        int64_t C, int64_t ldx, int64_t words, int64_t units) {
-  const int l16 = threadIdx.x & 15;
-  const int64_t row_bytes = mx_row_bytes(C);
-  const int64_t step = int64_t(gridDim.x) * (kMxThreads / 16);
-  // a whole warp stays in the loop together (the shuffles below name all lanes)
-  const int64_t first = int64_t(blockIdx.x) * (kMxThreads / 16) + (threadIdx.x >> 4);
-  for (int64_t u0 = first - ((threadIdx.x >> 4) & 1); u0 < units; u0 += step) {
-    const int64_t u = u0 + ((threadIdx.x >> 4) & 1);
-    const int64_t row = u / words, w = u - row * words;
-    const int64_t k = w * 128 + l16 * 8;
-    const bool live = u < units && row < R;
-    float v[8];
-    load8<T, VEC>(x + row * ldx + k, live ? C - k : 0, v);
+// Low or high 16-bit value of a word as fp32.
+template <typename T>
+__device__ __forceinline__ float half_of(uint32_t w, int high) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w);
+    return high ? __high2float(h) : __low2float(h);
+  } else {
+    return __uint_as_float(high ? w & 0xffff0000u : w << 16);
+  }
+}
+// The largest magnitude among `N` words, as fp32 bits (NaN above infinity): of 16-bit types both halves of a word
+// are compared at once.
+template <typename T, int N>
+__device__ __forceinline__ uint32_t top_of(const uint32_t* w) {
+  if constexpr (sizeof(T) == 4) {
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, mx_magnitude(v[i]));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t byte = mx_scale_byte(top);
-    const uint32_t codes = mx_encode8(v, byte);
-    if (live && k < row_bytes * 2) *reinterpret_cast<uint32_t*>(q + row * row_bytes + (k >> 1)) = codes;
-    uint32_t word = byte << (8 * (l16 >> 2));
-    word |= __shfl_xor_sync(0xffffffffu, word, 4);
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
-    if (l16 == 0 && u < units) *reinterpret_cast<uint32_t*>(scale + mx_scale_offset(row, w * 4, words)) = word;
+    for (int i = 0; i < N; ++i) top = max(top, w[i] & 0x7fffffffu);
+    return top;
+  } else {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+    return max(__float_as_uint(half_of<T>(top, 0)), __float_as_uint(half_of<T>(top, 1)));
   }
 }
 
-// Blocks down the columns of x [R, C]: row c of the result is column c of x.  A thread owns one
-// column and four blocks of it (128 rows of x): consecutive lanes read consecutive columns, and what
-// a thread writes is 64 contiguous bytes of codes and one word of scales.
-template <typename T>
-__global__ void __launch_bounds__(kMxThreads)
-mx_quantize_cols_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ scale, int64_t R,
-                        int64_t C, int64_t ldx, int64_t words, int64_t padded_cols) {
-  const int64_t c = int64_t(blockIdx.x) * kMxThreads + threadIdx.x;
-  if (c >= padded_cols) return;
-  const int64_t row_bytes = mx_row_bytes(R);
-  for (int64_t w = blockIdx.y; w < words; w += gridDim.y) {
-    uint32_t word = 0;
-    for (int b = 0; b < 4; ++b) {
-      const int64_t r0 = w * 128 + b * 32;
-      float v[32];
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        v[i] = c < C && r0 + i < R ? to_f32(x[(r0 + i) * ldx + c]) : 0.0f;
-        top = max(top, mx_magnitude(v[i]));
-      }
-      const uint32_t byte = mx_scale_byte(top);
-      uint32_t codes[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float(&part)[8] = *reinterpret_cast<const float(*)[8]>(v + 8 * i);
-        codes[i] = mx_encode8(part, byte);
-      }
-      if (c < C && r0 < R)
-        *reinterpret_cast<uint4*>(q + c * row_bytes + (r0 >> 1)) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-      word |= byte << (8 * b);
-    }
-    *reinterpret_cast<uint32_t*>(scale + mx_scale_offset(c, w * 4, words)) = word;
-  }
-}
-
-// A lane takes eight elements: one word of codes in, 16 or 32 bytes of values out.
+// Blocks along the rows of x [R, C].  A warp takes a row, or kRowChunk words of four scales of it (a word covers 128
+// elements): sixteen elements a lane, so a block's largest magnitude is a maximum over two lanes, the codes of a warp
+// leave as 256 contiguous bytes, and eight lanes make a word of scales.  A lane has the loads of UNROLL times 16
+// elements in flight.  The grid also covers the rows that pad the last band of 128, whose scale bytes are zero.
+constexpr int kRowChunk = 32;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kMxThreads)
-mx_dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scale, T* __restrict__ x, int64_t rows,
-                     int64_t K, int64_t ldx, int64_t words, int64_t units) {
-  const int64_t row_bytes = mx_row_bytes(K);
-  const int64_t per_row = row_bytes / 4;
-  for (int64_t u = int64_t(blockIdx.x) * kMxThreads + threadIdx.x; u < units; u += int64_t(gridDim.x) * kMxThreads) {
-    const int64_t row = u / per_row, k = (u - row * per_row) * 8;
-    float v[8];
-    mx_decode8(*reinterpret_cast<const uint32_t*>(q + row * row_bytes + (k >> 1)),
-               scale[mx_scale_offset(row, k / 32, words)], v);
-    T* dst = x + row * ldx + k;
-    if (VEC && k + 8 <= K) {
-      if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-        T h[8];
+mx_quantize_rows_kernel(const T* x, uint8_t* q, uint8_t* scale, int64_t R,
+                        int64_t C, int64_t ldx, int words, int64_t padded_rows) {
+  constexpr int UNROLL = sizeof(T) == 4 ? 1 : 2;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = int64_t(blockIdx.x) * (kMxThreads / 32) + (threadIdx.x >> 5);
+  if (row >= padded_rows) return;  // whole warps
+  const int64_t row_bytes = mx_row_bytes(C);
+  const bool live = row < R;
+  const int end = min(words, (int(blockIdx.y) + 1) * kRowChunk);
+  mx_follow_stream();
+  for (int w0 = int(blockIdx.y) * kRowChunk; w0 < end; w0 += 4 * UNROLL) {
+    Sixteen<T> raw[UNROLL];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = from_f32<T>(v[i]);
-        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(h);
+    for (int i = 0; i < UNROLL; ++i) {
+      const int64_t k = int64_t(w0 + 4 * i) * 128 + lane * 16;
+      load16<T, VEC>(x + row * ldx + k, live ? C - k : 0, raw[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) {
+      const int word = w0 + 4 * i + (lane >> 3);
+      const int64_t k = int64_t(w0 + 4 * i) * 128 + lane * 16;
+      uint32_t top = top_of<T, Sixteen<T>::WORDS>(raw[i].w);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      const uint32_t byte = mx_scale_byte(top);
+      uint2 codes;
+      if constexpr (sizeof(T) == 4) {
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(raw[i].w[j]);
+        codes = make_uint2(mx_encode8(v, byte), mx_encode8(v + 8, byte));
+      } else {
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = half_of<T>(raw[i].w[j / 2], j & 1);
+        codes = make_uint2(mx_encode8(v, byte), mx_encode8(v + 8, byte));
+      }
+      if (live && k < row_bytes * 2) *reinterpret_cast<uint2*>(q + row * row_bytes + (k >> 1)) = codes;
+      uint32_t four = byte << (4 * (lane & 6));
+      four |= __shfl_xor_sync(0xffffffffu, four, 2);
+      four |= __shfl_xor_sync(0xffffffffu, four, 4);
+      if ((lane & 7) == 0 && word < words)
+        *reinterpret_cast<uint32_t*>(scale + mx_scale_offset(row, int64_t(word) * 4, words)) = four;
+    }
+  }
+}
+
+// Blocks down the columns of x [R, C]: row c of the result is column c of x.  A CTA takes 256 rows of x (eight
+// blocks, one a warp) and 64 columns, two a lane: a warp reads whole 128-byte (fp32: 256-byte) pieces of 32
+// rows, a lane then has both of its columns' blocks in registers.  The codes meet in shared memory, from where a
+// column's 128 bytes leave as one line, and the scale bytes as words.  VEC: pairs of columns are aligned.
+constexpr int kColTileK = 256, kColTileC = 64;
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kMxThreads)
+mx_quantize_cols_kernel(const T* x, uint8_t* q, uint8_t* scale, int64_t R,
+                        int64_t C, int64_t ldx, int words) {
+  constexpr int WORDS = sizeof(T) == 4 ? 64 : 32;   // a word is a pair of 16-bit values or one of two fp32 values
+  __shared__ uint4 codes[kColTileC][9];             // 128 bytes of codes a column, and 16 that part the banks
+  __shared__ __align__(4) uint8_t bytes[kColTileC][8];  // scale bytes of a column's eight blocks
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row_bytes = mx_row_bytes(R);
+  const int64_t c = int64_t(blockIdx.x) * kColTileC + 2 * lane;
+  mx_follow_stream();
+  for (int64_t k0 = int64_t(blockIdx.y) * kColTileK; k0 < int64_t(words) * 128; k0 += int64_t(gridDim.y) * kColTileK) {
+    const int64_t r0 = k0 + warp * 32;
+    const T* src = x + r0 * ldx + c;
+    uint32_t raw[WORDS];  // fp32: row i's two values at i and 32 + i
+    if (VEC && c + 1 < C && r0 + 32 <= R) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i, src += ldx) {
+        if constexpr (sizeof(T) == 4) {
+          const uint2 u = __ldcg(reinterpret_cast<const uint2*>(src));
+          raw[i] = u.x;
+          raw[32 + i] = u.y;
+        } else {
+          raw[i] = __ldcg(reinterpret_cast<const uint32_t*>(src));
+        }
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (k + i < K) dst[i] = from_f32<T>(v[i]);
+      for (int i = 0; i < 32; ++i, src += ldx) {
+        const bool in = r0 + i < R;
+        if constexpr (sizeof(T) == 4) {
+          raw[i] = in && c < C ? __float_as_uint(src[0]) : 0u;
+          raw[32 + i] = in && c + 1 < C ? __float_as_uint(src[1]) : 0u;
+        } else {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+          raw[i] = (in && c < C ? uint32_t(h[0]) : 0u) | (in && c + 1 < C ? uint32_t(h[1]) << 16 : 0u);
+        }
+      }
+    }
+    uint32_t top[2];
+    if constexpr (sizeof(T) == 4) {
+      top[0] = top_of<T, 32>(raw);
+      top[1] = top_of<T, 32>(raw + 32);
+    } else {
+      uint32_t both = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) both = __vmaxu2(both, raw[i] & 0x7fff7fffu);
+      top[0] = __float_as_uint(half_of<T>(both, 0));
+      top[1] = __float_as_uint(half_of<T>(both, 1));
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t byte = mx_scale_byte(top[h]);
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if constexpr (sizeof(T) == 4) v[j] = __uint_as_float(raw[32 * h + 8 * i + j]);
+          else v[j] = half_of<T>(raw[8 * i + j], h);
+        }
+        w[i] = mx_encode8(v, byte);
+      }
+      codes[2 * lane + h][warp] = make_uint4(w[0], w[1], w[2], w[3]);
+      bytes[2 * lane + h][warp] = uint8_t(byte);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kColTileC * 8 / kMxThreads; ++i) {
+      const int u = i * kMxThreads + threadIdx.x, col = u >> 3, piece = u & 7;
+      const int64_t row = int64_t(blockIdx.x) * kColTileC + col, at = (k0 >> 1) + piece * 16;
+      if (row < C && at < row_bytes) *reinterpret_cast<uint4*>(q + row * row_bytes + at) = codes[col][piece];
+    }
+    if (threadIdx.x < 2 * kColTileC) {
+      const int col = threadIdx.x >> 1, half = threadIdx.x & 1;
+      const int64_t row = int64_t(blockIdx.x) * kColTileC + col, block = k0 / 32 + half * 4;
+      if (block < int64_t(words) * 4)
+        *reinterpret_cast<uint32_t*>(scale + mx_scale_offset(row, block, words)) =
+            *reinterpret_cast<const uint32_t*>(&bytes[col][half * 4]);
+    }
+    __syncthreads();
+  }
+}
+
+// A warp takes 4096 elements of a row.  VEC (16-byte aligned rows): a lane writes 16 bytes at a time, four or eight
+// elements.  Otherwise consecutive lanes take consecutive elements, so that what a warp stores is contiguous all the
+// same (eight elements a lane, stored one by one, cost six times as much).
+constexpr int kDeqChunk = 4096;
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kMxThreads)
+mx_dequantize_kernel(const uint8_t* q, const uint8_t* scale, T* x, int64_t rows,
+                     int64_t K, int64_t ldx, int words) {
+  constexpr int N = VEC ? 16 / int(sizeof(T)) : 1;  // neighbours a lane takes
+  constexpr int UNROLL = VEC ? 4 : 8;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = int64_t(blockIdx.x) * (kMxThreads / 32) + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const uint8_t* qr = q + row * mx_row_bytes(K);
+  const uint8_t* sr = scale + mx_scale_offset(row, 0, words);
+  T* xr = x + row * ldx;
+  const int64_t end = min(K, (int64_t(blockIdx.y) + 1) * kDeqChunk);
+  mx_follow_stream();
+  for (int64_t k0 = int64_t(blockIdx.y) * kDeqChunk + lane * N; k0 < end; k0 += 32 * N * UNROLL) {
+    uint32_t codes[UNROLL], byte[UNROLL];
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) {
+      const int64_t k = k0 + i * 32 * N;
+      codes[i] = byte[i] = 0;
+      if (k < end) {
+        if constexpr (N == 8) codes[i] = __ldcg(reinterpret_cast<const uint32_t*>(qr + (k >> 1)));
+        else if constexpr (N == 4) codes[i] = __ldcg(reinterpret_cast<const uint16_t*>(qr + (k >> 1)));
+        else codes[i] = uint32_t(qr[k >> 1]) >> (4 * (k & 1));
+        byte[i] = sr[(k >> 7) * 512 + ((k >> 5) & 3)];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) {
+      const int64_t k = k0 + i * 32 * N;
+      if (k >= end) break;
+      float v[8];
+      mx_decode8(codes[i], byte[i], v);
+      alignas(16) T h[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) h[j] = from_f32<T>(v[j]);
+      if (VEC && k + N <= K) {
+        *reinterpret_cast<uint4*>(xr + k) = *reinterpret_cast<const uint4*>(h);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (k + j < K) xr[k + j] = h[j];
+      }
     }
   }
+}
+
+// A launch that may begin its set-up before the kernel ahead of it in the stream has ended.
+template <typename... Args>
+int launch_following(void (*kernel)(Args...), dim3 grid, cudaStream_t stream, std::decay_t<Args>... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kMxThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent_launch_enabled() ? 1 : 0;
+  B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return B200_OK;
 }
 
 template <typename T>
 int quantize_t(const T* x, uint8_t* q, uint8_t* scale, int64_t R, int64_t C, int64_t ldx, int along, cudaStream_t stream) {
   if (along == 0) {
-    const int64_t words = (C + 127) / 128, units = (R + 127) / 128 * 128 * words;
-    const int64_t want = (units + kMxThreads / 16 - 1) / (kMxThreads / 16);
-    const int grid = int(want < 148 * 32 ? want : 148 * 32);
+    const int64_t words = (C + 127) / 128, padded = (R + 127) / 128 * 128, chunks = (words + kRowChunk - 1) / kRowChunk;
+    if (chunks > 65535) return fail(B200_ERR_TOO_LARGE, "quantize_mxfp4: rows longer than %lld", 65535LL * kRowChunk * 128);
+    const dim3 grid(unsigned(padded / (kMxThreads / 32)), unsigned(chunks));
     const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * int64_t(sizeof(T)) % 16 == 0;
-    if (vec) mx_quantize_rows_kernel<T, true><<<grid, kMxThreads, 0, stream>>>(x, q, scale, R, C, ldx, words, units);
-    else mx_quantize_rows_kernel<T, false><<<grid, kMxThreads, 0, stream>>>(x, q, scale, R, C, ldx, words, units);
-  } else {
-    const int64_t words = (R + 127) / 128, padded = (C + 127) / 128 * 128;
-    dim3 grid(unsigned((padded + kMxThreads - 1) / kMxThreads), unsigned(words < 65535 ? words : 65535));
-    mx_quantize_cols_kernel<T><<<grid, kMxThreads, 0, stream>>>(x, q, scale, R, C, ldx, words, padded);
+    return launch_following(vec ? mx_quantize_rows_kernel<T, true> : mx_quantize_rows_kernel<T, false>, grid, stream, x, q,
+                            scale, R, C, ldx, int(words), padded);
   }
-  B200_CUDA_TRY(cudaGetLastError());
-  return B200_OK;
+  const int64_t words = (R + 127) / 128, padded = (C + 127) / 128 * 128, tall = (words * 128 + kColTileK - 1) / kColTileK;
+  const dim3 grid(unsigned(padded / kColTileC), unsigned(tall < 65535 ? tall : 65535));
+  const bool vec = reinterpret_cast<uintptr_t>(x) % (2 * sizeof(T)) == 0 && ldx % 2 == 0;
+  return launch_following(vec ? mx_quantize_cols_kernel<T, true> : mx_quantize_cols_kernel<T, false>, grid, stream, x, q,
+                          scale, R, C, ldx, int(words));
 }
 
 template <typename T>
 int dequantize_t(const uint8_t* q, const uint8_t* scale, T* x, int64_t rows, int64_t K, int64_t ldx, cudaStream_t stream) {
-  const int64_t words = (K + 127) / 128, units = rows * (mx_row_bytes(K) / 4);
-  const int64_t want = (units + kMxThreads - 1) / kMxThreads;
-  const int grid = int(want < 148 * 32 ? want : 148 * 32);
+  const int64_t words = (K + 127) / 128, chunks = (K + kDeqChunk - 1) / kDeqChunk;
+  if (chunks > 65535) return fail(B200_ERR_TOO_LARGE, "dequantize_mxfp4: rows longer than %lld", 65535LL * kDeqChunk);
+  const dim3 grid(unsigned((rows + kMxThreads / 32 - 1) / (kMxThreads / 32)), unsigned(chunks));
   const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * int64_t(sizeof(T)) % 16 == 0;
-  if (vec) mx_dequantize_kernel<T, true><<<grid, kMxThreads, 0, stream>>>(q, scale, x, rows, K, ldx, words, units);
-  else mx_dequantize_kernel<T, false><<<grid, kMxThreads, 0, stream>>>(q, scale, x, rows, K, ldx, words, units);
-  B200_CUDA_TRY(cudaGetLastError());
-  return B200_OK;
+  return launch_following(vec ? mx_dequantize_kernel<T, true> : mx_dequantize_kernel<T, false>, grid, stream, q, scale, x,
+                          rows, K, ldx, int(words));
 }
 
 bool float_dtype(int dtype) { return dtype == B200_F16 || dtype == B200_BF16 || dtype == B200_F32; }

@@ -30,11 +30,8 @@ __host__ __device__ __forceinline__ int64_t mx_scale_offset(int64_t row, int64_t
   return ((row >> 7) * words + (block >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
 }
 
-// |v| as an integer that orders like the magnitude, with NaN above infinity: a maximum over a block
-// keeps what is not finite in sight.
-__device__ __forceinline__ uint32_t mx_magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
-// Scale byte of a block whose largest magnitude has the bits `top`: the element format's largest power
+// Scale byte of a block whose largest magnitude has the fp32 bits `top` (taken as an integer maximum, which keeps NaN
+// and infinity in sight): the element format's largest power
 // of two is 4, so the exponent is floor(log2 max) - 2, kept at -127 and above (zero blocks too).  A block
 // with an infinity or a NaN in it gets 255, the scale format's NaN.
 __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t top) {
@@ -45,19 +42,16 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t top) {
 // Codes of eight elements under a scale byte, element i in bits [4i, 4i + 4): x / 2^E rounded to nearest,
 // ties to the even code, magnitudes beyond 6 taken to 6.  1 / 2^E is a normal fp32 number for every
 // byte up to 253, so the product is exact wherever it does not vanish.
-__device__ __forceinline__ uint32_t mx_encode8(const float (&v)[8], uint32_t byte) {
+__device__ __forceinline__ uint32_t mx_encode8(const float* v, uint32_t byte) {
   if (byte == 255u) return 0u;
   const float inv = __uint_as_float((254u - byte) << 23);
-  uint32_t r = 0;
+  uint32_t pair[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t pair;
+  for (int i = 0; i < 4; ++i)
     asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\tcvt.u32.u8 %0, b;\n\t}"
-        : "=r"(pair)
+        : "=r"(pair[i])
         : "f"(v[2 * i + 1] * inv), "f"(v[2 * i] * inv));
-    r |= pair << (8 * i);
-  }
-  return r;
+  return __byte_perm(__byte_perm(pair[0], pair[1], 0x0040), __byte_perm(pair[2], pair[3], 0x0040), 0x5410);
 }
 
 // Value of a scale byte: 2^(byte - 127); 0 is a subnormal fp32 number, 255 is NaN.
