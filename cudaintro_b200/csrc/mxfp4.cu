@@ -36,10 +36,10 @@ struct Sixteen {
   static constexpr int WORDS = 4 * sizeof(T);
   uint32_t w[WORDS];
 };
-// Elements at or beyond `left` (how many the row still has) are 0.  VEC: the address is 16-byte aligned.
-template <typename T, bool VEC>
+// The address is 16-byte aligned; elements at or beyond `left` (how many the row still has) are 0.
+template <typename T>
 __device__ __forceinline__ void load16(const T* src, int64_t left, Sixteen<T>& v) {
-  if (VEC && left >= 16) {
+  if (left >= 16) {
 #pragma unroll
     for (int i = 0; i < Sixteen<T>::WORDS / 4; ++i) {
       const uint4 u = __ldcg(reinterpret_cast<const uint4*>(src) + i);
@@ -56,6 +56,41 @@ __device__ __forceinline__ void load16(const T* src, int64_t left, Sixteen<T>& v
       }
     }
   }
+}
+
+// A warp's copy of `n` (at most 512) neighbours that are aligned to their element size only, into aligned shared memory;
+// zeros up to 512.  16-bit elements are read as aligned words, the first element on its own where the address asks
+// for it: consecutive lanes read consecutive words whatever the alignment.
+template <typename T>
+__device__ __forceinline__ void stage512(const T* src, int n, T* dst, int lane) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t r[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int e = i * 32 + lane;
+      r[i] = e < n ? reinterpret_cast<const uint32_t*>(src)[e] : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) reinterpret_cast<uint32_t*>(dst)[i * 32 + lane] = r[i];
+  } else {
+    const int odd = int(reinterpret_cast<uintptr_t>(src) >> 1) & 1;
+    const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src);
+    uint16_t* d16 = reinterpret_cast<uint16_t*>(dst);
+    uint32_t r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = odd + 2 * (i * 32 + lane);  // the word holds elements e and e + 1
+      r[i] = e + 1 < n ? *reinterpret_cast<const uint32_t*>(s16 + e) : e < n ? uint32_t(s16[e]) : 0u;
+    }
+    if (odd && lane == 0) d16[0] = n > 0 ? s16[0] : uint16_t(0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = odd + 2 * (i * 32 + lane);
+      d16[e] = uint16_t(r[i]);
+      if (e + 1 < 512) d16[e + 1] = uint16_t(r[i] >> 16);
+    }
+  }
+  __syncwarp();
 }
 
 // Low or high 16-bit value of a word as fp32.
@@ -94,7 +129,8 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kMxThreads)
 mx_quantize_rows_kernel(const T* x, uint8_t* q, uint8_t* scale, int64_t R,
                         int64_t C, int64_t ldx, int words, int64_t padded_rows) {
-  constexpr int UNROLL = sizeof(T) == 4 ? 1 : 2;
+  constexpr int UNROLL = sizeof(T) == 4 || !VEC ? 1 : 2;
+  __shared__ alignas(16) T stage[VEC ? 1 : kMxThreads / 32][VEC ? 1 : 512];
   const int lane = threadIdx.x & 31;
   const int64_t row = int64_t(blockIdx.x) * (kMxThreads / 32) + (threadIdx.x >> 5);
   if (row >= padded_rows) return;  // whole warps
@@ -107,7 +143,16 @@ mx_quantize_rows_kernel(const T* x, uint8_t* q, uint8_t* scale, int64_t R,
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {
       const int64_t k = int64_t(w0 + 4 * i) * 128 + lane * 16;
-      load16<T, VEC>(x + row * ldx + k, live ? C - k : 0, raw[i]);
+      if constexpr (VEC) {
+        load16(x + row * ldx + k, live ? C - k : 0, raw[i]);
+      } else {
+        const int64_t k0 = int64_t(w0) * 128;
+        T* buf = stage[threadIdx.x >> 5];
+        __syncwarp();
+        stage512(x + row * ldx + k0, live ? int(min(C - k0, int64_t(512))) : 0, buf, lane);
+#pragma unroll
+        for (int j = 0; j < Sixteen<T>::WORDS; ++j) raw[i].w[j] = reinterpret_cast<const uint32_t*>(buf)[lane * Sixteen<T>::WORDS + j];
+      }
     }
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {
@@ -144,7 +189,7 @@ mx_quantize_rows_kernel(const T* x, uint8_t* q, uint8_t* scale, int64_t R,
 // column's 128 bytes leave as one line, and the scale bytes as words.  VEC: pairs of columns are aligned.
 constexpr int kColTileK = 256, kColTileC = 64;
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kMxThreads)
+__global__ void __launch_bounds__(kMxThreads, sizeof(T) == 4 ? 2 : 3)
 mx_quantize_cols_kernel(const T* x, uint8_t* q, uint8_t* scale, int64_t R,
                         int64_t C, int64_t ldx, int words) {
   constexpr int WORDS = sizeof(T) == 4 ? 64 : 32;   // a word is a pair of 16-bit values or one of two fp32 values
@@ -228,52 +273,76 @@ mx_quantize_cols_kernel(const T* x, uint8_t* q, uint8_t* scale, int64_t R,
   }
 }
 
-// A warp takes 4096 elements of a row.  VEC (16-byte aligned rows): a lane writes 16 bytes at a time, four or eight
-// elements.  Otherwise consecutive lanes take consecutive elements, so that what a warp stores is contiguous all the
-// same (eight elements a lane, stored one by one, cost six times as much).
+// A warp takes kDeqChunk elements of a row, a lane 16 bytes of values (eight or four elements) at a time.  VEC (16-byte
+// aligned rows): they are stored as such.  Otherwise the values of 32 x 16 bytes meet in shared memory and leave as words,
+// consecutive lanes consecutive words (stored from the lanes' registers, element by element, rows of 11007 16-bit
+// values cost 142 us where these take 28).
 constexpr int kDeqChunk = 4096;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kMxThreads)
-mx_dequantize_kernel(const uint8_t* q, const uint8_t* scale, T* x, int64_t rows,
-                     int64_t K, int64_t ldx, int words) {
-  constexpr int N = VEC ? 16 / int(sizeof(T)) : 1;  // neighbours a lane takes
-  constexpr int UNROLL = VEC ? 4 : 8;
+mx_dequantize_kernel(const uint8_t* q, const uint8_t* scale, T* x, int64_t rows, int64_t K, int64_t ldx, int words) {
+  constexpr int N = 16 / int(sizeof(T));  // neighbours a lane takes
+  constexpr int UNROLL = 4;
+  __shared__ alignas(16) T stage[VEC ? 1 : kMxThreads / 32][VEC ? 1 : 32 * N];
   const int lane = threadIdx.x & 31;
   const int64_t row = int64_t(blockIdx.x) * (kMxThreads / 32) + (threadIdx.x >> 5);
-  if (row >= rows) return;
+  if (row >= rows) return;  // whole warps
   const uint8_t* qr = q + row * mx_row_bytes(K);
   const uint8_t* sr = scale + mx_scale_offset(row, 0, words);
   T* xr = x + row * ldx;
   const int64_t end = min(K, (int64_t(blockIdx.y) + 1) * kDeqChunk);
   mx_follow_stream();
-  for (int64_t k0 = int64_t(blockIdx.y) * kDeqChunk + lane * N; k0 < end; k0 += 32 * N * UNROLL) {
+  for (int64_t first = int64_t(blockIdx.y) * kDeqChunk; first < end; first += 32 * N * UNROLL) {
     uint32_t codes[UNROLL], byte[UNROLL];
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {
-      const int64_t k = k0 + i * 32 * N;
+      const int64_t k = first + (i * 32 + lane) * N;
       codes[i] = byte[i] = 0;
       if (k < end) {
         if constexpr (N == 8) codes[i] = __ldcg(reinterpret_cast<const uint32_t*>(qr + (k >> 1)));
-        else if constexpr (N == 4) codes[i] = __ldcg(reinterpret_cast<const uint16_t*>(qr + (k >> 1)));
-        else codes[i] = uint32_t(qr[k >> 1]) >> (4 * (k & 1));
+        else codes[i] = __ldcg(reinterpret_cast<const uint16_t*>(qr + (k >> 1)));
         byte[i] = sr[(k >> 7) * 512 + ((k >> 5) & 3)];
       }
     }
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {
-      const int64_t k = k0 + i * 32 * N;
-      if (k >= end) break;
+      const int64_t k0 = first + i * 32 * N, k = k0 + lane * N;
+      if (k0 >= end) break;  // the whole warp
       float v[8];
       mx_decode8(codes[i], byte[i], v);
       alignas(16) T h[N];
 #pragma unroll
       for (int j = 0; j < N; ++j) h[j] = from_f32<T>(v[j]);
-      if (VEC && k + N <= K) {
-        *reinterpret_cast<uint4*>(xr + k) = *reinterpret_cast<const uint4*>(h);
-      } else {
+      if constexpr (VEC) {
+        if (k + N <= K) {
+          *reinterpret_cast<uint4*>(xr + k) = *reinterpret_cast<const uint4*>(h);
+        } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (k + j < K) xr[k + j] = h[j];
+          for (int j = 0; j < N; ++j)
+            if (k + j < K) xr[k + j] = h[j];
+        }
+      } else {
+        T* buf = stage[threadIdx.x >> 5];
+        *reinterpret_cast<uint4*>(buf + lane * N) = *reinterpret_cast<const uint4*>(h);
+        __syncwarp();
+        const int n = int(min(K - k0, int64_t(32 * N)));
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            if (j * 32 + lane < n) xr[k0 + j * 32 + lane] = buf[j * 32 + lane];
+        } else {
+          const uint16_t* b16 = reinterpret_cast<const uint16_t*>(buf);
+          uint16_t* d16 = reinterpret_cast<uint16_t*>(xr + k0);
+          const int odd = int(reinterpret_cast<uintptr_t>(d16) >> 1) & 1;
+          if (odd && lane == 0) d16[0] = b16[0];
+#pragma unroll
+          for (int j = 0; j < N / 2; ++j) {
+            const int e = odd + 2 * (j * 32 + lane);
+            if (e + 1 < n) *reinterpret_cast<uint32_t*>(d16 + e) = uint32_t(b16[e]) | (uint32_t(b16[e + 1]) << 16);
+            else if (e < n) d16[e] = b16[e];
+          }
+        }
+        __syncwarp();
       }
     }
   }
