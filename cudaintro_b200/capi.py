@@ -373,11 +373,11 @@ def linear_mxfp4(x, w, w_scale, bias=None, relu=False, out=None):
                                  and bias.get_device() == index):
         raise ValueError(f"bias: a contiguous fp32 tensor [{out_f}] on {x.device}")
     out = _mx_out(out, batch, out_f, x.dtype, x)
-    need = batch * (K >> 1) + ((batch + 127) >> 7) * ((K + 127) >> 7) * 512
-    ws = x.new_empty(need, dtype=torch.uint8)
+    need = lib.b200_linear_mxfp4_workspace(batch, in_f)
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
     _mx_call(index, lib.b200_linear_mxfp4, code, x.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
              None if bias is None else bias.data_ptr(), out.data_ptr(), batch, in_f, out_f, LINEAR_RELU if relu else 0,
-             ws.data_ptr(), need)
+             None if ws is None else ws.data_ptr(), need)
     return out
 
 

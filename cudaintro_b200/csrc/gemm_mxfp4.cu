@@ -67,32 +67,43 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, budget_ns)) != 0;
 }
 
+// Shared-memory descriptors are handed over as their address word alone; the upper words are constants.  kOperandHi:
+// rows of 128 bytes, 128-byte swizzle, 1024 bytes between groups of eight rows.  kScaleHi: lines of 16 bytes without a
+// swizzle, 128 bytes between groups of eight.
+constexpr uint32_t kOperandHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+constexpr uint32_t kScaleHi = (128u >> 4) | (1u << 14);
+__device__ __forceinline__ uint32_t desc_word(uint32_t smem_addr) { return ((smem_addr & 0x3ffffu) >> 4) | (1u << 16); }
+
 template <int CG>
-__device__ __forceinline__ void mx_umma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa_tmem,
+__device__ __forceinline__ void mx_umma(uint32_t d_tmem, uint32_t a_desc, uint32_t b_desc, uint32_t idesc, uint32_t sa_tmem,
                                         uint32_t sb_tmem, uint32_t accumulate) {
   if constexpr (CG == 2)
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %7};\n\tmov.b64 b, {%2, %7};\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [%4], [%5], p;\n\t}"
         :
-        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+        : "r"(d_tmem), "r"(a_desc), "r"(b_desc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate), "n"(kOperandHi)
         : "memory");
   else
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %7};\n\tmov.b64 b, {%2, %7};\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [%4], [%5], p;\n\t}"
         :
-        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+        : "r"(d_tmem), "r"(a_desc), "r"(b_desc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate), "n"(kOperandHi)
         : "memory");
 }
 
 // One scale tile, shared memory -> four columns of tensor memory (of both CTAs of a pair, each from its own).
 template <int CG>
-__device__ __forceinline__ void mx_copy_scales(uint32_t tmem, uint64_t desc) {
+__device__ __forceinline__ void mx_copy_scales(uint32_t tmem, uint32_t desc) {
   if constexpr (CG == 2)
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    asm volatile("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\ttcgen05.cp.cta_group::2.32x128b.warpx4 [%0], d;\n\t}" ::"r"(tmem),
+                 "r"(desc), "n"(kScaleHi)
+                 : "memory");
   else
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    asm volatile("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\ttcgen05.cp.cta_group::1.32x128b.warpx4 [%0], d;\n\t}" ::"r"(tmem),
+                 "r"(desc), "n"(kScaleHi)
+                 : "memory");
 }
 
 // 3-D tiled load, credited to a barrier of either CTA of a pair (CG = 2) or of this CTA.
@@ -128,7 +139,8 @@ struct MxTile {
   static constexpr int STAGING_BYTES = kEpiWarps * 32 * 128;
   static constexpr int STAGES_FIT = (kSmemBudget - 2048 - STAGING_BYTES) / STAGE_BYTES;
   static constexpr int STAGES = STAGES_FIT > 6 ? 6 : STAGES_FIT;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + STAGING_BYTES + 1024 + 256;
+  static_assert(STAGES * STAGE_BYTES + STAGING_BYTES + 1024 + 256 <= kSmemBudget, "shared memory");
+  static constexpr int SMEM_BYTES = kSmemBudget;  // all of it: who owns all of tensor memory shares the SM with nobody
   static constexpr int ACC_STEP = BN == 256 ? 192 : BN;  // columns from accumulator 0 to accumulator 1
   static constexpr int SCALE_COL = 448;                  // first column of the scale buffers
   static constexpr int SCALE_STEP = 32;                  // columns of one buffer: 8 for A, 8 x BANDS for B
@@ -292,11 +304,10 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     if (cta_rank == 0) {
       constexpr uint32_t idesc0 = mx_instr_desc(T::TILE_M, BN, 0), idesc2 = mx_instr_desc(T::TILE_M, BN, 2);
       const uint32_t ring = smem_u32(smem);
-      const uint64_t a_desc0 = make_smem_desc_sw128(ring, 16, 1024);
-      const uint64_t b_desc0 = make_smem_desc_sw128(ring + T::A_BYTES, 16, 1024);
-      // scale tiles: 8 x 16-byte core matrices, 128 bytes apart, no swizzle
-      const uint64_t s_desc0 = make_smem_desc(ring + T::A_BYTES + T::B_BYTES, 16, 128, 0);
-      constexpr uint64_t kStageStep = uint64_t(T::STAGE_BYTES >> 4);
+      const uint32_t a_desc0 = desc_word(ring);
+      const uint32_t b_desc0 = desc_word(ring + T::A_BYTES);
+      const uint32_t s_desc0 = desc_word(ring + T::A_BYTES + T::B_BYTES);
+      constexpr uint32_t kStageStep = T::STAGE_BYTES >> 4;
       int stage = 0, behind = 0;  // `behind`: the stage of the k-block before the last
       uint32_t phase = 0, behind_phase = 0, count = 0;
       bool ok = true;
@@ -315,23 +326,23 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           tc_fence_after_sync();
           const uint32_t sa_tmem = tmem_base + uint32_t(T::SCALE_COL) + (count & 1u) * uint32_t(T::SCALE_STEP);
           const uint32_t sb_tmem = sa_tmem + 8;
-          const uint64_t s_desc = s_desc0 + uint64_t(stage) * kStageStep;
-          const uint64_t a_desc = a_desc0 + uint64_t(stage) * kStageStep;
-          const uint64_t b_desc = b_desc0 + uint64_t(stage) * kStageStep;
+          const uint32_t s_desc = s_desc0 + uint32_t(stage) * kStageStep;
+          const uint32_t a_desc = a_desc0 + uint32_t(stage) * kStageStep;
+          const uint32_t b_desc = b_desc0 + uint32_t(stage) * kStageStep;
           const int left = p.blocks - kb * 8;  // blocks of 32 this stage really holds
           if (elect_lane()) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              mx_copy_scales<CG>(sa_tmem + uint32_t(4 * h), s_desc + uint64_t((h * kScaleTile) >> 4));
+              mx_copy_scales<CG>(sa_tmem + uint32_t(4 * h), s_desc + uint32_t((h * kScaleTile) >> 4));
 #pragma unroll
               for (int b = 0; b < T::BANDS; ++b)
                 mx_copy_scales<CG>(sb_tmem + uint32_t(h * 4 * T::BANDS + 4 * b),
-                                   s_desc + uint64_t((T::SA_BYTES + (2 * b + h) * kScaleTile) >> 4));
+                                   s_desc + uint32_t((T::SA_BYTES + (2 * b + h) * kScaleTile) >> 4));
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               if (2 * j < left)
-                mx_umma<CG>(d_tmem, a_desc + uint64_t(2 * j), b_desc + uint64_t(2 * j), (j & 1) ? idesc2 : idesc0,
+                mx_umma<CG>(d_tmem, a_desc + uint32_t(2 * j), b_desc + uint32_t(2 * j), (j & 1) ? idesc2 : idesc0,
                             sa_tmem + uint32_t(4 * (j >> 1)), sb_tmem + uint32_t(4 * T::BANDS * (j >> 1)),
                             (kb | j) != 0 ? 1u : 0u);
             }
@@ -441,6 +452,303 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   }
 }
 
+// ------------------------------------------------------------------------------ few rows of A
+//
+// A product of at most 128 rows of A streams B (the weights) and computes little.  Here the weights are the 128-row
+// operand of the MMA and the rows of A ("tokens", padded to 16) its N dimension, so no instruction is spent on rows
+// that do not exist, and an accumulator lane is one output feature.  A tile of 128 features is shared by a cluster of
+// S CTAs, one range of K each, so that every SM streams; the partial sums meet through distributed shared
+// memory: each CTA of the cluster finishes 128 / S features, adding the ranges in K order.
+//
+// SRC = 1, 2, 3: the tokens arrive as fp32, fp16 or bf16 rows and six warps quantise this CTA's range of them into
+// shared memory, in the order the MMA reads, while the weights are on their way: one launch for a layer.
+// SRC = 0: they arrive packed and travel through the ring with the weights.
+//
+// Warp 0 issues the loads, warp 1 the scale copies and MMAs, warps 2-7 quantise, all take part in the tail.  The scale
+// buffers in tensor memory are those of the ring's stages, so a buffer is rewritten only after the stage's MMAs.
+
+enum { SRC_PACKED = 0, SRC_F32 = 1, SRC_F16 = 2, SRC_BF16 = 3 };
+constexpr int kSkQuantWarps = 14;
+__host__ __device__ constexpr int sk_threads(int src) { return src == SRC_PACKED ? 256 : 64 + 32 * kSkQuantWarps; }
+constexpr int kSkMaxStages = 12;
+constexpr int kSkMaxPieces = 16;  // pieces of 512 elements in a CTA's range of a token
+// Rows of A the kernel takes.  Measured against the general kernel (128 x 128 tiles), us: [11008, 4096] weights, 1 row
+// 7.2 / 12.8, 16 rows 9.0 / 12.6, 32 rows 10.7 / 12.6, 64 rows 15.7 / 10.3 (86 tiles, two ranges of K); [4096, 11008], 64
+// rows 14.0 / 19.6, 128 rows 22.4 / 20.0 (32 tiles, four ranges); [1024, 2048], 48 rows 7.4 / 5.9 (eight ranges of one
+// k-block).  So: up to 32 rows always, up to 64 where K is cut in four or more and at least 4096 long.
+constexpr int kSkRows = 32, kSkMaxRows = 64, kSkLongK = 4096;
+// Rows that the kernel quantises itself: 16 rows of 11008 into 4096 features take 12.0 us in one launch (8.5 of them the
+// product's, the quantising is done again by every tile of features), 15 us in two; 32 rows 21 us in one, 15.4 in two.
+constexpr int kSkFusedRows = 16;
+constexpr int64_t kSkFusedK = 65536;      // ... and their length: an eighth of it fits in shared memory
+constexpr int kWeightBytes = 128 * 128;     // 128 features x 256 elements
+constexpr int kWeightScales = 2 * kScaleTile;
+
+struct MxSkinnyArgs {
+  void* C;
+  const void* X;  // rows of A as they are (SRC != 0)
+  int64_t ldc;
+  int M, N, K;
+  int blocks;          // blocks of 32 along K
+  int tokens;          // M rounded up to 16
+  int splits;          // CTAs of a cluster = ranges of K
+  int kb_per_split;    // k-blocks (256 elements) per range; the last range may be shorter, never empty
+  int stages;
+  int tmem_cols;
+  int scale_col;       // first column of the scale buffers (16 columns each)
+  int x_vec;           // rows of X are 16-byte aligned
+  const float* bias;
+  int relu;
+  unsigned long long wait_budget_ns;
+  int lose_kb;
+};
+
+template <int SRC> struct SkSource { using type = float; };
+template <> struct SkSource<SRC_F16> { using type = __half; };
+template <> struct SkSource<SRC_BF16> { using type = __nv_bfloat16; };
+
+__device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+
+template <int EPI>
+__device__ __forceinline__ void sk_store(const MxSkinnyArgs& p, int m, int n, float y) {
+  if (p.bias != nullptr) y += p.bias[n];
+  if (p.relu) y = fmaxf(0.0f, y);
+  const int64_t at = int64_t(m) * p.ldc + n;
+  if constexpr (EPI == EPI_F32) static_cast<float*>(p.C)[at] = y;
+  else if constexpr (EPI == EPI_F16) static_cast<__half*>(p.C)[at] = __float2half_rn(y);
+  else static_cast<__nv_bfloat16*>(p.C)[at] = __float2bfloat16_rn(y);
+}
+
+template <int SRC, int EPI>
+__global__ void __launch_bounds__(sk_threads(SRC), 2)
+gemm_mx_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_sw,
+                      const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_sx,
+                      const MxSkinnyArgs p) {
+  using X = typename SkSource<SRC>::type;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int tokens = p.tokens, S = p.splits;
+  const int token_bytes = tokens * 128;  // one k-block of the tokens
+  // ring: weights | tokens (packed source only) | weight scales | token scales (packed source only)
+  const int stage_bytes = kWeightBytes + kWeightScales + (SRC == SRC_PACKED ? token_bytes + 2 * kScaleTile : 0);
+  const int scale_ofs = kWeightBytes + (SRC == SRC_PACKED ? token_bytes : 0);
+  uint8_t* xq = smem + p.stages * stage_bytes;  // quantised tokens: [k-block][tokens][128 bytes], then their scales
+  uint8_t* xs = xq + (SRC == SRC_PACKED ? 0 : p.kb_per_split * token_bytes);
+  float* exch = reinterpret_cast<float*>(xs + (SRC == SRC_PACKED ? 0 : p.kb_per_split * 2 * kScaleTile));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(exch) + (S > 1 ? 128 * tokens * 4 : 0));
+  uint64_t* empty_bar = full_bar + kSkMaxStages;
+  uint64_t* acc_full = empty_bar + kSkMaxStages;
+  uint64_t* x_ready = acc_full + 1;  // [kSkMaxPieces]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_ready + kSkMaxPieces);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = S > 1 ? cluster_cta_rank() : 0u;
+  const int tile = int(blockIdx.x) / S;
+  const int n0 = tile * 128;
+  const int num_kb = (p.blocks + 7) / 8;
+  const int kb0 = int(rank) * p.kb_per_split;
+  const int kb_count = min(p.kb_per_split, num_kb - kb0);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    if constexpr (SRC != SRC_PACKED)
+      for (int i = 0; i < kSkMaxPieces; ++i) mbar_init(&x_ready[i], uint32_t(p.M));
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_sw);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, uint32_t(p.tmem_cols));
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncwarp();
+  if (S > 1) cluster_sync_all(); else __syncthreads();  // every CTA of the cluster runs from here on
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ loads
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < kb_count; ++i) {
+      if (!warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_budget_ns)) break;
+      const int kb = kb0 + i;
+      const bool lost = kb == p.lose_kb && blockIdx.x == 0;
+      if (!lost && elect_lane()) {
+        uint8_t* sw = smem + stage * stage_bytes;
+        uint8_t* ss = sw + scale_ofs;
+        mbar_arrive_expect_tx(&full_bar[stage], uint32_t(stage_bytes));
+        tma_load_2d(sw, &tmap_w, &full_bar[stage], kb * 128, n0);
+        mx_load_3d<1>(ss, &tmap_sw, smem_u32(&full_bar[stage]), 0, kb * 2, tile);
+        if constexpr (SRC == SRC_PACKED) {
+          tma_load_2d(sw + kWeightBytes, &tmap_x, &full_bar[stage], kb * 128, 0);
+          mx_load_3d<1>(ss + kWeightScales, &tmap_sx, smem_u32(&full_bar[stage]), 0, kb * 2, 0);
+        }
+      }
+      __syncwarp();
+      if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ scale copies and MMAs
+    const uint32_t idesc0 = mx_instr_desc(128, tokens, 0), idesc2 = mx_instr_desc(128, tokens, 2);
+    const uint32_t ring = smem_u32(smem);
+    const uint32_t w_desc0 = desc_word(ring);
+    const uint32_t x_desc0 = desc_word(SRC == SRC_PACKED ? ring + kWeightBytes : smem_u32(xq));
+    const uint32_t sw_desc0 = desc_word(ring + uint32_t(scale_ofs));
+    const uint32_t sx_desc0 = desc_word(SRC == SRC_PACKED ? ring + uint32_t(scale_ofs + kWeightScales) : smem_u32(xs));
+    const uint32_t w_step = uint32_t(stage_bytes >> 4);
+    const uint32_t x_step = SRC == SRC_PACKED ? w_step : uint32_t(token_bytes >> 4);
+    const uint32_t sx_step = SRC == SRC_PACKED ? w_step : uint32_t((2 * kScaleTile) >> 4);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int i = 0; i < kb_count && ok; ++i) {
+      if constexpr (SRC != SRC_PACKED) {
+        if ((i & 1) == 0 && !warp_wait(&x_ready[i >> 1], 0, abort_flag, p.wait_budget_ns)) { ok = false; break; }
+      }
+      if (!warp_wait(&full_bar[stage], phase, abort_flag, p.wait_budget_ns)) { ok = false; break; }
+      tc_fence_after_sync();
+      const int at = SRC == SRC_PACKED ? stage : i;
+      const uint32_t sa_tmem = tmem_base + uint32_t(p.scale_col + stage * 16);
+      const uint32_t sb_tmem = sa_tmem + 8;
+      const uint32_t w_desc = w_desc0 + uint32_t(stage) * w_step, sw_desc = sw_desc0 + uint32_t(stage) * w_step;
+      const uint32_t x_desc = x_desc0 + uint32_t(at) * x_step, sx_desc = sx_desc0 + uint32_t(at) * sx_step;
+      const int left = p.blocks - (kb0 + i) * 8;
+      if (elect_lane()) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          mx_copy_scales<1>(sa_tmem + uint32_t(4 * h), sw_desc + uint32_t((h * kScaleTile) >> 4));
+          mx_copy_scales<1>(sb_tmem + uint32_t(4 * h), sx_desc + uint32_t((h * kScaleTile) >> 4));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (2 * j < left)
+            mx_umma<1>(tmem_base, w_desc + uint32_t(2 * j), x_desc + uint32_t(2 * j), (j & 1) ? idesc2 : idesc0,
+                       sa_tmem + uint32_t(4 * (j >> 1)), sb_tmem + uint32_t(4 * (j >> 1)), (i | j) != 0 ? 1u : 0u);
+        }
+        umma_commit(&empty_bar[stage]);
+        if (i + 1 == kb_count) umma_commit(acc_full);
+      }
+      __syncwarp();
+      if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+    }
+  } else if constexpr (SRC != SRC_PACKED) {
+    // ------------------------------------------------------------------ tokens -> shared memory
+    // A warp takes 512 elements (a piece, two k-blocks) of a token at a time, sixteen a lane, two lanes a block, with the
+    // loads of UNROLL tokens in flight.  The first piece of all tokens comes first, so that its MMAs can start.
+    constexpr int UNROLL = 2;
+    const X* x = static_cast<const X*>(p.X);
+    const int pieces = (kb_count + 1) / 2;
+    const int piece_step = kSkQuantWarps / p.M, m_step = kSkQuantWarps - piece_step * p.M;
+    int piece_next = (warp - 2) / p.M, m_next = (warp - 2) - piece_next * p.M;
+    while (piece_next < pieces) {
+      Sixteen<X> raw[UNROLL];
+      int at_m[UNROLL], at_e[UNROLL];
+#pragma unroll
+      for (int i = 0; i < UNROLL; ++i) {
+        at_m[i] = m_next;
+        at_e[i] = piece_next * 512 + lane * 16;
+        const int64_t k = int64_t(kb0) * 256 + at_e[i];
+        load16(x + int64_t(m_next) * p.K + k, piece_next < pieces ? p.K - k : 0, raw[i], p.x_vec != 0);
+        piece_next += piece_step;
+        m_next += m_step;
+        if (m_next >= p.M) {
+          m_next -= p.M;
+          ++piece_next;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < UNROLL; ++i) {
+        const int m = at_m[i], e = at_e[i];
+        uint32_t top = top_of<X, Sixteen<X>::WORDS>(raw[i].w);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        const uint32_t byte = mx_scale_byte(top);
+        const uint2 codes = encode16(raw[i], byte);
+        uint32_t four = byte << (4 * (lane & 6));
+        four |= __shfl_xor_sync(0xffffffffu, four, 2);
+        four |= __shfl_xor_sync(0xffffffffu, four, 4);
+        const int kb = e >> 8;  // k-block within this CTA's range
+        if (kb < kb_count) {
+          // 128-byte swizzle: 16-byte chunk c of row m lies at chunk c ^ (m % 8)
+          const int in_row = (e & 255) >> 1, chunk = (in_row >> 4) ^ (m & 7);
+          *reinterpret_cast<uint2*>(xq + kb * token_bytes + m * 128 + (chunk << 4) + (in_row & 15)) = codes;
+          if ((lane & 7) == 0)
+            *reinterpret_cast<uint32_t*>(xs + kb * 2 * kScaleTile + ((e >> 7) & 1) * kScaleTile + (m & 31) * 16 + (m >> 5) * 4) = four;
+        }
+      }
+      fence_proxy_async_smem();  // the MMAs and scale copies read what was written here
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < UNROLL; ++i)
+        if (lane == 0 && (at_e[i] >> 9) < pieces) mbar_arrive(&x_ready[at_e[i] >> 9]);
+    }
+  }
+  __syncwarp();
+
+  // Tail: an accumulator lane is a feature, a column a token.  The warps that share a quarter of the lanes take sixteen
+  // tokens each in turn.
+  const int quarter = warp & 3, feature = quarter * 32 + lane;
+  const int own = 128 / S;  // features a CTA of the cluster finishes
+  const bool acc_ready = warp_wait(acc_full, 0, abort_flag, p.wait_budget_ns);
+  tc_fence_after_sync();
+  if (acc_ready) {
+    const uint32_t dst_cta = S > 1 ? map_to_cta(smem_u32(exch), uint32_t(feature / own)) : 0u;
+    for (int m0 = (warp >> 2) * 16; m0 < p.M; m0 += sk_threads(SRC) / 8) {
+      uint32_t v[16];
+      tmem_ld_32x16(tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(m0), v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (m0 + i < p.M) {
+          if (S > 1) st_cluster_u32(dst_cta + uint32_t(((int(rank) * tokens + m0 + i) * own + feature % own) * 4), v[i]);
+          else if (n0 + feature < p.N) sk_store<EPI>(p, m0 + i, n0 + feature, __uint_as_float(v[i]));
+        }
+      }
+    }
+  }
+  __syncwarp();
+  if (S > 1) {
+    cluster_sync_all();  // every range's sums have arrived, and nobody writes into another CTA after this
+    if (*abort_flag == 0u) {
+      const int first = n0 + int(rank) * own;
+      for (int i = threadIdx.x; i < own * p.M; i += sk_threads(SRC)) {
+        const int m = i / own, f = i - m * own;
+        if (first + f < p.N) {
+          float y = exch[m * own + f];
+          for (int r = 1; r < S; ++r) y += exch[(r * tokens + m) * own + f];
+          sk_store<EPI>(p, m, first + f, y);
+        }
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0) atomicOr(&g_mx_status, 2u);
+    // Give copies and MMAs still in flight time to land before shared and tensor memory go away.
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, uint32_t(p.tmem_cols));
+  }
+}
+
 // ------------------------------------------------------------------------------ host side
 
 // Packed elements as bytes: 128-byte swizzle, zeros outside the matrix.
@@ -529,11 +837,140 @@ int launch_tile(const MxGemm& g, int sms, cudaStream_t stream) {
   return B200_OK;
 }
 
+struct SkinnyPlan {
+  int splits = 0, per = 0, stages = 0, smem = 0, tokens = 0, tmem_cols = 0;
+};
+
+// Several of these CTAs share an SM, and a CTA that finds no room in tensor memory waits in tcgen05.alloc without a
+// limit while its cluster waits for it.  So a CTA's share of an SM's shared memory (1 KB of which the system takes)
+// is never below its share of the 512 columns: CTAs that fit together in the one fit in the other, whatever
+// launches they come from.
+constexpr int kSmSharedBytes = 228 * 1024;
+int skinny_tmem_cols(int tokens, int stages) {
+  int cols = 32;
+  while (cols < tokens + 16 * stages) cols *= 2;
+  return cols;
+}
+int skinny_smem(bool packed, int tokens, int per, int splits, int stages) {
+  const int stage = kWeightBytes + kWeightScales + (packed ? tokens * 128 + 2 * kScaleTile : 0);
+  const int need = stages * stage + (packed ? 0 : per * (tokens * 128 + 2 * kScaleTile)) +
+                   (splits > 1 ? 128 * tokens * 4 : 0) + 1024 + 512;
+  const int share = skinny_tmem_cols(tokens, stages) * (kSmSharedBytes / 512) - 1024;
+  return need > share ? need : share;
+}
+
+// Cluster size: the largest that asks for at most a quarter more CTAs than there are SMs.  Measured, 1 / 2 / 4 / 8 ranges, us:
+// one row, [11008, 4096] (86 tiles) 9.7 / 8.5 / 13.3 / 14.0; 8 rows, [4096, 4096] (32 tiles) 12.4 / 9.9 / 7.4 / 8.7; 16 rows,
+// [4096, 11008] packed 15.9 / 12.1 / 8.8 / 9.3.
+SkinnyPlan plan_skinny(const MxGemm& g, bool packed, int sms) {
+  SkinnyPlan best;
+  const int num_kb = int((g.K + 255) / 256), tokens = int((g.M + 15) / 16) * 16;
+  const int64_t tiles = (g.N + 127) / 128;
+  for (int s = 1; s <= 8; s *= 2) {
+    if (best.splits && tiles * s * 4 > int64_t(sms) * 5) break;
+    const int per = (num_kb + s - 1) / s;
+    if ((num_kb + per - 1) / per != s) continue;  // a range would be empty
+    // a ring that leaves room for a second CTA on the SM, another cluster's or the next launch's (with all of the SM's
+    // memory one row of the 86-tile layer takes 13.9 us instead of 8.4)
+    int stages = per < kSkMaxStages ? per : kSkMaxStages;
+    while (stages > 2 && skinny_smem(packed, tokens, per, s, stages) > kSmSharedBytes / 2 - 1024) --stages;
+    const int smem = skinny_smem(packed, tokens, per, s, stages);
+    if (smem > kSmemBudget || (!packed && (per + 1) / 2 > kSkMaxPieces)) continue;
+    best.splits = s;
+    best.per = per;
+    best.stages = stages;
+    best.smem = smem;
+    best.tokens = tokens;
+    best.tmem_cols = skinny_tmem_cols(tokens, stages);
+  }
+  return best;
+}
+
+template <int SRC, int EPI>
+int launch_skinny(const MxGemm& g, const SkinnyPlan& plan, cudaStream_t stream) {
+  auto kernel = gemm_mx_skinny_kernel<SRC, EPI>;
+  static thread_local int last_dev = -1;
+  int dev = 0;
+  B200_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev != last_dev) {
+    B200_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget));
+    last_dev = dev;
+  }
+  MxSkinnyArgs p;
+  memset(&p, 0, sizeof(p));
+  p.C = g.C;
+  p.X = g.X;
+  p.ldc = g.ldc;
+  p.M = int(g.M);
+  p.N = int(g.N);
+  p.K = int(g.K);
+  p.blocks = int((g.K + 31) / 32);
+  p.tokens = plan.tokens;
+  p.splits = plan.splits;
+  p.kb_per_split = plan.per;
+  p.stages = plan.stages;
+  p.scale_col = plan.tokens;
+  p.tmem_cols = plan.tmem_cols;
+  p.bias = g.tail.bias;
+  p.relu = g.tail.flags & B200_LINEAR_RELU;
+  wait_test_settings(&p.lose_kb, &p.wait_budget_ns);
+  const int64_t row_bytes = mx_row_bytes(g.K), tiles_k = (g.K + 127) / 128;
+  CUtensorMap mw, msw, mx, msx;
+  int rc = map_elements(&mw, g.B, g.N, row_bytes, 128);
+  if (!rc) rc = map_scales(&msw, g.b_scale, g.N, tiles_k, 1);
+  if (rc) return rc;
+  if (SRC == SRC_PACKED) {
+    rc = map_elements(&mx, g.A, g.M, row_bytes, plan.tokens);
+    if (!rc) rc = map_scales(&msx, g.a_scale, g.M, tiles_k, 1);
+    if (rc) return rc;
+  } else {
+    const int64_t pitch = g.K * (SRC == SRC_F32 ? 4 : 2);
+    p.x_vec = pitch % 16 == 0 && reinterpret_cast<uintptr_t>(g.X) % 16 == 0;
+    memset(&mx, 0, sizeof(mx));
+    memset(&msx, 0, sizeof(msx));
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned((g.N + 127) / 128 * plan.splits));
+  cfg.blockDim = dim3(unsigned(sk_threads(SRC)));
+  cfg.dynamicSmemBytes = size_t(plan.smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int nattr = 0;
+  if (dependent_launch_enabled()) {
+    attr[nattr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[nattr].val.programmaticStreamSerializationAllowed = 1;
+    ++nattr;
+  }
+  if (plan.splits > 1) {
+    attr[nattr].id = cudaLaunchAttributeClusterDimension;
+    attr[nattr].val.clusterDim.x = unsigned(plan.splits);
+    attr[nattr].val.clusterDim.y = 1;
+    attr[nattr].val.clusterDim.z = 1;
+    ++nattr;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = unsigned(nattr);
+  B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, mw, msw, mx, msx, p));
+  return B200_OK;
+}
+
+int device_sms(int* sms) {
+  int dev = 0;
+  B200_CUDA_TRY(cudaGetDevice(&dev));
+  B200_CUDA_TRY(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+  return B200_OK;
+}
+
 template <int EPI>
 int launch_epi(const MxGemm& g, cudaStream_t stream) {
-  int dev = 0, sms = 0;
-  B200_CUDA_TRY(cudaGetDevice(&dev));
-  B200_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  int sms = 0;
+  int rc = device_sms(&sms);
+  if (rc) return rc;
+  if (g.M <= kSkMaxRows) {
+    const SkinnyPlan plan = plan_skinny(g, true, sms);
+    if (plan.splits && (g.M <= kSkRows || (plan.splits >= 4 && g.K >= kSkLongK)))
+      return launch_skinny<SRC_PACKED, EPI>(g, plan, stream);
+  }
   // CTA pairs once they give every pair of SMs a tile.
   const int64_t pair_tiles = ((g.M + 255) / 256) * ((g.N + 255) / 256);
   if (g.M > 128 && pair_tiles >= sms / 2) return launch_tile<2, 256, EPI>(g, sms, stream);
@@ -547,6 +984,21 @@ int launch_mx_gemm(int out_dtype, const MxGemm& g, cudaStream_t stream) {
     case B200_F32: return launch_epi<EPI_F32>(g, stream);
     case B200_F16: return launch_epi<EPI_F16>(g, stream);
     default: return launch_epi<EPI_BF16>(g, stream);
+  }
+}
+
+bool mx_layer_in_one_launch(int64_t rows, int64_t K) { return rows <= kSkFusedRows && K <= kSkFusedK; }
+
+int launch_mx_layer(int dtype, const MxGemm& g, cudaStream_t stream) {
+  int sms = 0;
+  int rc = device_sms(&sms);
+  if (rc) return rc;
+  const SkinnyPlan plan = plan_skinny(g, false, sms);
+  if (!plan.splits) return fail(B200_ERR_TOO_LARGE, "linear_mxfp4: in_features %lld", (long long)g.K);
+  switch (dtype) {
+    case B200_F32: return launch_skinny<SRC_F32, EPI_F32>(g, plan, stream);
+    case B200_F16: return launch_skinny<SRC_F16, EPI_F16>(g, plan, stream);
+    default: return launch_skinny<SRC_BF16, EPI_BF16>(g, plan, stream);
   }
 }
 

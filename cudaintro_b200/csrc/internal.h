@@ -73,6 +73,9 @@ int encode_tiled_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const
 // Product of two 4-bit matrices (gemm_mxfp4.cu); out_dtype is B200_F32, B200_F16 or B200_BF16.
 struct MxGemm;
 int launch_mx_gemm(int out_dtype, const MxGemm& g, cudaStream_t stream);
+// The layer on rows that are not quantised yet, in one launch; for the products that mx_layer_in_one_launch accepts.
+bool mx_layer_in_one_launch(int64_t rows, int64_t K);
+int launch_mx_layer(int dtype, const MxGemm& g, cudaStream_t stream);
 int read_and_clear_mx_status(uint32_t* out);
 
 // What set_wait_test left: the k-block to lose (-1 = none) and the limit of a single wait.

@@ -30,34 +30,6 @@ __device__ __forceinline__ void mx_follow_stream() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// Sixteen neighbours of a row, as they lie in memory: words of two 16-bit values, or of one fp32 value.
-template <typename T>
-struct Sixteen {
-  static constexpr int WORDS = 4 * sizeof(T);
-  uint32_t w[WORDS];
-};
-// The address is 16-byte aligned; elements at or beyond `left` (how many the row still has) are 0.
-template <typename T>
-__device__ __forceinline__ void load16(const T* src, int64_t left, Sixteen<T>& v) {
-  if (left >= 16) {
-#pragma unroll
-    for (int i = 0; i < Sixteen<T>::WORDS / 4; ++i) {
-      const uint4 u = __ldcg(reinterpret_cast<const uint4*>(src) + i);
-      v.w[4 * i] = u.x; v.w[4 * i + 1] = u.y; v.w[4 * i + 2] = u.z; v.w[4 * i + 3] = u.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if constexpr (sizeof(T) == 4) {
-        v.w[i] = i < left ? __float_as_uint(src[i]) : 0u;
-      } else {
-        const uint32_t e = i < left ? reinterpret_cast<const uint16_t*>(src)[i] : 0u;
-        v.w[i / 2] = i & 1 ? v.w[i / 2] | (e << 16) : e;
-      }
-    }
-  }
-}
-
 // A warp's copy of `n` (at most 512) neighbours that are aligned to their element size only, into aligned shared memory;
 // zeros up to 512.  16-bit elements are read as aligned words, the first element on its own where the address asks
 // for it: consecutive lanes read consecutive words whatever the alignment.
@@ -91,33 +63,6 @@ __device__ __forceinline__ void stage512(const T* src, int n, T* dst, int lane) 
     }
   }
   __syncwarp();
-}
-
-// Low or high 16-bit value of a word as fp32.
-template <typename T>
-__device__ __forceinline__ float half_of(uint32_t w, int high) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 h = *reinterpret_cast<const __half2*>(&w);
-    return high ? __high2float(h) : __low2float(h);
-  } else {
-    return __uint_as_float(high ? w & 0xffff0000u : w << 16);
-  }
-}
-// The largest magnitude among `N` words, as fp32 bits (NaN above infinity): of 16-bit types both halves of a word
-// are compared at once.
-template <typename T, int N>
-__device__ __forceinline__ uint32_t top_of(const uint32_t* w) {
-  if constexpr (sizeof(T) == 4) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) top = max(top, w[i] & 0x7fffffffu);
-    return top;
-  } else {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
-    return max(__float_as_uint(half_of<T>(top, 0)), __float_as_uint(half_of<T>(top, 1)));
-  }
 }
 
 // Blocks along the rows of x [R, C].  A warp takes a row, or kRowChunk words of four scales of it (a word covers 128
@@ -161,18 +106,7 @@ mx_quantize_rows_kernel(const T* x, uint8_t* q, uint8_t* scale, int64_t R,
       uint32_t top = top_of<T, Sixteen<T>::WORDS>(raw[i].w);
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       const uint32_t byte = mx_scale_byte(top);
-      uint2 codes;
-      if constexpr (sizeof(T) == 4) {
-        float v[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(raw[i].w[j]);
-        codes = make_uint2(mx_encode8(v, byte), mx_encode8(v + 8, byte));
-      } else {
-        float v[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = half_of<T>(raw[i].w[j / 2], j & 1);
-        codes = make_uint2(mx_encode8(v, byte), mx_encode8(v + 8, byte));
-      }
+      const uint2 codes = encode16(raw[i], byte);
       if (live && k < row_bytes * 2) *reinterpret_cast<uint2*>(q + row * row_bytes + (k >> 1)) = codes;
       uint32_t four = byte << (4 * (lane & 6));
       four |= __shfl_xor_sync(0xffffffffu, four, 2);
@@ -484,7 +418,7 @@ extern "C" int b200_gemm_mxfp4(int out_dtype, const void* A, const void* a_scale
 }
 
 extern "C" size_t b200_linear_mxfp4_workspace(int64_t batch, int64_t in_features) {
-  if (batch <= 0 || in_features <= 0) return 0;
+  if (batch <= 0 || in_features <= 0 || mx_layer_in_one_launch(batch, in_features)) return 0;
   return b200_mxfp4_scale_bytes(batch, in_features) + size_t(batch) * b200_mxfp4_row_bytes(in_features);
 }
 
@@ -499,18 +433,8 @@ extern "C" int b200_linear_mxfp4(int dtype, const void* X, const void* W, const 
   if (flags & ~(B200_LINEAR_RELU | B200_LINEAR_BIAS_FIRST)) return fail(B200_ERR_BAD_ARGUMENT, "unknown flags 0x%x", flags);
   if (bias && reinterpret_cast<uintptr_t>(bias) % 4)
     return fail(B200_ERR_UNSUPPORTED, "linear_mxfp4: bias is not aligned to its element size");
-  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16)
-    return fail(B200_ERR_BAD_ARGUMENT, "linear_mxfp4: the workspace must be given, 16-byte aligned");
-  const size_t need = b200_linear_mxfp4_workspace(batch, in_features);
-  if (workspace_bytes < need)
-    return fail(B200_ERR_BAD_ARGUMENT, "linear_mxfp4: the workspace has %zu bytes, %zu are needed", workspace_bytes, need);
-  uint8_t* s = static_cast<uint8_t*>(workspace);
-  uint8_t* q = s + b200_mxfp4_scale_bytes(batch, in_features);
-  rc = quantize(dtype, X, q, s, batch, in_features, in_features, 0, stream);
-  if (rc) return rc;
   MxGemm g;
-  g.A = q;
-  g.a_scale = s;
+  g.X = X;
   g.B = static_cast<const uint8_t*>(W);
   g.b_scale = static_cast<const uint8_t*>(w_scale);
   g.C = Y;
@@ -520,5 +444,17 @@ extern "C" int b200_linear_mxfp4(int dtype, const void* X, const void* W, const 
   g.ldc = out_features;
   g.tail.bias = bias;
   g.tail.flags = flags;
+  const size_t need = b200_linear_mxfp4_workspace(batch, in_features);
+  if (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return fail(B200_ERR_BAD_ARGUMENT, "linear_mxfp4: the workspace must be given, 16-byte aligned");
+  if (workspace_bytes < need)
+    return fail(B200_ERR_BAD_ARGUMENT, "linear_mxfp4: the workspace has %zu bytes, %zu are needed", workspace_bytes, need);
+  if (!need) return launch_mx_layer(dtype, g, stream);
+  uint8_t* s = static_cast<uint8_t*>(workspace);
+  uint8_t* q = s + b200_mxfp4_scale_bytes(batch, in_features);
+  rc = quantize(dtype, X, q, s, batch, in_features, in_features, 0, stream);
+  if (rc) return rc;
+  g.A = q;
+  g.a_scale = s;
   return launch_mx_gemm(dtype, g, stream);
 }

@@ -1,8 +1,11 @@
 // The MXFP4 format on the device: scale bytes, element codes, and where a scale byte lies.
 #pragma once
 
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "internal.h"
 
@@ -10,7 +13,8 @@ namespace b200 {
 
 // A product of two 4-bit matrices, C[M,N] = A[M,K] * B[N,K]^T, with the optional tail of a layer.
 struct MxGemm {
-  const uint8_t* A = nullptr;
+  const uint8_t* A = nullptr;  // or X, rows that are yet to be quantised (launch_mx_layer)
+  const void* X = nullptr;
   const uint8_t* a_scale = nullptr;
   const uint8_t* B = nullptr;
   const uint8_t* b_scale = nullptr;
@@ -70,6 +74,73 @@ __device__ __forceinline__ void mx_decode8(uint32_t codes, uint32_t byte, float 
     v[2 * i] = f.x * s;
     v[2 * i + 1] = f.y * s;
   }
+}
+
+// Sixteen neighbours of a row, as they lie in memory: words of two 16-bit values, or of one fp32 value.
+template <typename T>
+struct Sixteen {
+  static constexpr int WORDS = 4 * sizeof(T);
+  uint32_t w[WORDS];
+};
+// The address is 16-byte aligned if `vec`; elements at or beyond `left` (how many the row still has) are 0.
+template <typename T>
+__device__ __forceinline__ void load16(const T* src, int64_t left, Sixteen<T>& v, bool vec = true) {
+  if (vec && left >= 16) {
+#pragma unroll
+    for (int i = 0; i < Sixteen<T>::WORDS / 4; ++i) {
+      const uint4 u = __ldcg(reinterpret_cast<const uint4*>(src) + i);
+      v.w[4 * i] = u.x; v.w[4 * i + 1] = u.y; v.w[4 * i + 2] = u.z; v.w[4 * i + 3] = u.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        v.w[i] = i < left ? __float_as_uint(src[i]) : 0u;
+      } else {
+        const uint32_t e = i < left ? reinterpret_cast<const uint16_t*>(src)[i] : 0u;
+        v.w[i / 2] = i & 1 ? v.w[i / 2] | (e << 16) : e;
+      }
+    }
+  }
+}
+
+// Low or high 16-bit value of a word as fp32.
+template <typename T>
+__device__ __forceinline__ float half_of(uint32_t w, int high) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w);
+    return high ? __high2float(h) : __low2float(h);
+  } else {
+    return __uint_as_float(high ? w & 0xffff0000u : w << 16);
+  }
+}
+// The largest magnitude among `N` words, as fp32 bits (NaN above infinity): of 16-bit types both halves of a word
+// are compared at once.
+template <typename T, int N>
+__device__ __forceinline__ uint32_t top_of(const uint32_t* w) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = max(top, w[i] & 0x7fffffffu);
+    return top;
+  } else {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+    return max(__float_as_uint(half_of<T>(top, 0)), __float_as_uint(half_of<T>(top, 1)));
+  }
+}
+
+// Codes of sixteen elements under a scale byte.
+template <typename T>
+__device__ __forceinline__ uint2 encode16(const Sixteen<T>& x, uint32_t byte) {
+  float v[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    if constexpr (sizeof(T) == 4) v[j] = __uint_as_float(x.w[j]);
+    else v[j] = half_of<T>(x.w[j / 2], j & 1);
+  }
+  return make_uint2(mx_encode8(v, byte), mx_encode8(v + 8, byte));
 }
 
 }  // namespace b200

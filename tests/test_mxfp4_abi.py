@@ -17,7 +17,8 @@ def test_sizes_of_packed_arrays(cb):
     assert lib.b200_mxfp4_scale_bytes(129, 128) == 1024 and lib.b200_mxfp4_scale_bytes(129, 129) == 2048
     assert lib.b200_mxfp4_scale_bytes(0, 5) == 0 and lib.b200_mxfp4_scale_bytes(5, -1) == 0
     assert lib.b200_mxfp4_scale_bytes(1 << 30, 1 << 30) == 1 << 55  # no 32-bit wrap
-    assert lib.b200_linear_mxfp4_workspace(33, 784) >= 33 * 400 + 7 * 512
+    assert lib.b200_linear_mxfp4_workspace(200, 784) >= 200 * 400 + 14 * 512
+    assert lib.b200_linear_mxfp4_workspace(1, 4096) == 0 and lib.b200_linear_mxfp4_workspace(1, 1 << 20) > 0
     assert lib.b200_linear_mxfp4_workspace(0, 784) == 0
 
 
@@ -49,7 +50,7 @@ def test_refusals(cb):
     def gemm(dtype=bf16, a=one, sa=one, b=one, sb=one, c=one, M=4, N=4, K=64, ldc=0):
         return lib.b200_gemm_mxfp4(dtype, a, sa, b, sb, c, M, N, K, ldc, None)
 
-    def linear(dtype=bf16, x=one, w=one, sw=one, bias=None, y=one, batch=4, i=64, o=4, flags=0, ws=one, n=1 << 20):
+    def linear(dtype=bf16, x=one, w=one, sw=one, bias=None, y=one, batch=200, i=64, o=4, flags=0, ws=one, n=1 << 20):
         return lib.b200_linear_mxfp4(dtype, x, w, sw, bias, y, batch, i, o, flags, ws, n, None)
 
     big = (1 << 30) + 1
@@ -60,7 +61,7 @@ def test_refusals(cb):
         (gemm, [dict(dtype=i8), dict(a=None), dict(sa=None), dict(b=None), dict(sb=None), dict(c=None), dict(M=0), dict(N=0),
                 dict(K=0), dict(ldc=3)]),
         (linear, [dict(dtype=i8), dict(x=None), dict(w=None), dict(sw=None), dict(y=None), dict(batch=0), dict(i=0), dict(o=0),
-                  dict(flags=4), dict(ws=None), dict(n=0), dict(n=lib.b200_linear_mxfp4_workspace(4, 64) - 1), dict(ws=odd)]),
+                  dict(flags=4), dict(ws=None), dict(n=0), dict(n=lib.b200_linear_mxfp4_workspace(200, 64) - 1), dict(ws=odd)]),
     ):
         for kw in wrong:
             assert call(**kw) == 1, (call.__name__, kw)
