@@ -397,37 +397,48 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           }
         }
         if (n0 >= p.N) continue;
-        if (p.tma_store) {
 #pragma unroll
-          for (int box = 0; box < 64 / BOX_COLS; ++box) {
-            uint32_t w[32];
-            mx_finish<EPI>(p, n0 + box * BOX_COLS, v[box], w);
-            if constexpr (EPI != EPI_F32) mx_finish<EPI>(p, n0 + 32, v[1], w + 16);
-            if (lane == 0) tma_store_wait_read<0>();  // this warp's previous store has read the buffer
-            __syncwarp();
+        for (int box = 0; box < 64 / BOX_COLS; ++box) {
+          const int c0 = n0 + box * BOX_COLS;
+          uint32_t w[32];
+          mx_finish<EPI>(p, c0, v[box], w);
+          if constexpr (EPI != EPI_F32) mx_finish<EPI>(p, n0 + 32, v[1], w + 16);
+          if (p.tma_store && lane == 0) tma_store_wait_read<0>();  // this warp's previous store has read the buffer
+          __syncwarp();
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-              *reinterpret_cast<uint4*>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) =
-                  make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+          for (int u = 0; u < 8; ++u)
+            *reinterpret_cast<uint4*>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) =
+                make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+          if (p.tma_store) {
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0 && row0 < p.M && n0 + box * BOX_COLS < p.N) {
-              tma_store_2d(&tmap_c, buf, n0 + box * BOX_COLS, row0);
+            if (lane == 0 && row0 < p.M && c0 < p.N) {
+              tma_store_2d(&tmap_c, buf, c0, row0);
               tma_store_commit();
             }
-          }
-        } else if (row0 + lane < p.M) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t w[32];
-            mx_finish<EPI>(p, n0 + 32 * h, v[h], w);
-            char* crow = static_cast<char*>(p.C) + (int64_t(row0 + lane) * p.ldc + n0 + 32 * h) * OUT_BYTES;
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (n0 + 32 * h + e < p.N) {
-                if constexpr (EPI == EPI_F32) reinterpret_cast<uint32_t*>(crow)[e] = w[e];
-                else reinterpret_cast<uint16_t*>(crow)[e] = uint16_t(w[e >> 1] >> ((e & 1) * 16));
+          } else {
+            // C or its rows are not 16-byte aligned: the warp writes the box row by row, consecutive lanes
+            // consecutive words; a row of 16-bit values that begins in the middle of a word gives its first value
+            // on its own.  (Each lane storing its own row, element by element: 230 us for 951 x 23085, this LLL.)
+            __syncwarp();
+            const int rows = min(32, p.M - row0), cols = min(BOX_COLS, p.N - c0);
+            char* crow = static_cast<char*>(p.C) + (int64_t(row0) * p.ldc + c0) * OUT_BYTES;
+            for (int r = 0; r < rows; ++r, crow += p.ldc * OUT_BYTES) {
+              const uint8_t* line = buf + r * 128;
+              auto at = [&](int byte) { return line + ((((byte >> 4) ^ r) & 7) << 4) + (byte & 15); };
+              if constexpr (EPI == EPI_F32) {
+                if (lane < cols) reinterpret_cast<uint32_t*>(crow)[lane] = *reinterpret_cast<const uint32_t*>(at(4 * lane));
+              } else {
+                const int odd = int(reinterpret_cast<uintptr_t>(crow) >> 1) & 1, e = odd + 2 * lane;
+                uint16_t* c16 = reinterpret_cast<uint16_t*>(crow);
+                const uint32_t lo = e < 64 ? *reinterpret_cast<const uint16_t*>(at(2 * e)) : 0u;
+                const uint32_t hi = e + 1 < 64 ? *reinterpret_cast<const uint16_t*>(at(2 * e + 2)) : 0u;
+                if (e + 1 < cols) *reinterpret_cast<uint32_t*>(c16 + e) = lo | (hi << 16);
+                else if (e < cols) c16[e] = uint16_t(lo);
+                if (odd && lane == 0) c16[0] = *reinterpret_cast<const uint16_t*>(at(0));
               }
+            }
+            __syncwarp();
           }
         }
       }
@@ -479,7 +490,9 @@ constexpr int kSkMaxPieces = 16;  // pieces of 512 elements in a CTA's range of 
 constexpr int kSkRows = 32, kSkMaxRows = 64, kSkLongK = 4096;
 // Rows that the kernel quantises itself: 16 rows of 11008 into 4096 features take 12.0 us in one launch (8.5 of them the
 // product's, the quantising is done again by every tile of features), 15 us in two; 32 rows 21 us in one, 15.4 in two.
+// What the quantising costs a CTA goes with rows x its range, so up to 64 short rows are taken too.
 constexpr int kSkFusedRows = 16;
+constexpr int64_t kSkFusedElements = 65536;
 constexpr int64_t kSkFusedK = 65536;      // ... and their length: an eighth of it fits in shared memory
 constexpr int kWeightBytes = 128 * 128;     // 128 features x 256 elements
 constexpr int kWeightScales = 2 * kScaleTile;
@@ -987,7 +1000,9 @@ int launch_mx_gemm(int out_dtype, const MxGemm& g, cudaStream_t stream) {
   }
 }
 
-bool mx_layer_in_one_launch(int64_t rows, int64_t K) { return rows <= kSkFusedRows && K <= kSkFusedK; }
+bool mx_layer_in_one_launch(int64_t rows, int64_t K) {
+  return K <= kSkFusedK && (rows <= kSkFusedRows || (rows <= kSkMaxRows && rows * K <= kSkFusedElements));
+}
 
 int launch_mx_layer(int dtype, const MxGemm& g, cudaStream_t stream) {
   int sms = 0;
