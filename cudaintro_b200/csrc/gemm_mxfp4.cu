@@ -136,7 +136,7 @@ struct MxTile {
   static constexpr int SA_BYTES = 2 * kScaleTile;
   static constexpr int SB_BYTES = BANDS * 2 * kScaleTile;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;
-  static constexpr int STAGING_BYTES = kEpiWarps * 32 * 128;
+  static constexpr int STAGING_BYTES = kEpiWarps * (32 * 128 + 128 * 4);  // a box of 32 rows x 128 bytes and 128 values of the bias
   static constexpr int STAGES_FIT = (kSmemBudget - 2048 - STAGING_BYTES) / STAGE_BYTES;
   static constexpr int STAGES = STAGES_FIT > 6 ? 6 : STAGES_FIT;
   static_assert(STAGES * STAGE_BYTES + STAGING_BYTES + 1024 + 256 <= kSmemBudget, "shared memory");
@@ -154,7 +154,7 @@ struct MxArgs {
   int M, N;
   int blocks;  // blocks of 32 along K
   int tiles_m, tiles_n, group_m;
-  int tma_store;
+  int tma_store;  // C and its rows are 16-byte aligned
   const float* bias;
   int relu;
   unsigned long long wait_budget_ns;
@@ -169,13 +169,19 @@ __device__ __forceinline__ void mx_tile_coords(int t, const MxArgs& p, int& mb, 
   nb = r / gm;
 }
 
-// 32 accumulators of one row -> 32 (fp32) or 16 output words, with the tail.
+// 32 accumulators of one row -> 32 (fp32) or 16 output words, with the tail; `bias`: the 32 columns' values.
 template <int EPI>
-__device__ __forceinline__ void mx_finish(const MxArgs& p, int n0, uint32_t (&v)[32], uint32_t* w) {
+__device__ __forceinline__ void mx_finish(const MxArgs& p, const float* bias, uint32_t (&v)[32],
+                                          uint32_t (&w)[EPI == EPI_F32 ? 32 : 16]) {
   if (p.bias != nullptr) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      v[i] = __float_as_uint(__uint_as_float(v[i]) + p.bias[min(n0 + i, p.N - 1)]);
+    for (int i = 0; i < 8; ++i) {
+      const float4 b = reinterpret_cast<const float4*>(bias)[i];
+      v[4 * i] = __float_as_uint(__uint_as_float(v[4 * i]) + b.x);
+      v[4 * i + 1] = __float_as_uint(__uint_as_float(v[4 * i + 1]) + b.y);
+      v[4 * i + 2] = __float_as_uint(__uint_as_float(v[4 * i + 2]) + b.z);
+      v[4 * i + 3] = __float_as_uint(__uint_as_float(v[4 * i + 3]) + b.w);
+    }
   }
   if (p.relu) {
 #pragma unroll
@@ -359,15 +365,29 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   } else {
     // ------------------------------------------------------------------ epilogue
     constexpr int OUT_BYTES = EPI == EPI_F32 ? 4 : 2;
-    constexpr int BOX_COLS = 128 / OUT_BYTES;
+    constexpr int HALF_CHUNKS = 32 * OUT_BYTES / 16;  // 16-byte chunks of 32 outputs of a row
+    constexpr int BOX_COLS = 128 / OUT_BYTES;         // a box: 32 rows of 128 bytes
+    constexpr int MINE = T::UNITS / 2;
     const int group = (warp - 2) >> 2;  // two warps per quarter share a tile's units of 64 columns
     const int quarter = warp & 3;       // tensor-memory lanes this warp may read
-    uint8_t* buf = staging + (warp - 2) * (32 * 128);
+    uint8_t* box = staging + (warp - 2) * (32 * 128);
+    float* bias_buf = reinterpret_cast<float*>(staging + kEpiWarps * 32 * 128) + (warp - 2) * 128;
+    auto box_at = [&](int row, int byte) { return box + row * 128 + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15); };
     int it = 0;
     for (int t = first_tile; t < num_tiles; t += tile_step, ++it) {
       int mb, nb;
       mx_tile_coords(t, p, mb, nb);
       const int ab = it & 1;
+      // Group 0 begins with the unit that the other accumulator overlaps (the last one of accumulator 0, the first one
+      // of accumulator 1); group 1 has the units between.
+      auto unit_of = [&](int i) { return T::UNITS == 2 ? group : (group == 0 ? ((i ^ ab) ? 0 : 3) : 1 + i); };
+      if (p.bias != nullptr) {  // on its way while the tile is computed
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 2 * MINE; ++i)
+          bias_buf[32 * i + lane] = p.bias[min(nb * BN + unit_of(i >> 1) * 64 + (i & 1) * 32 + lane, p.N - 1)];
+        __syncwarp();
+      }
       volatile uint32_t* epi_go = epi_go_pair + (it & 1);
       // One warp polls the barrier; all eight agree on the outcome.
       if (warp == 2) {
@@ -378,16 +398,13 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       if (*epi_go == 0u) break;
       tc_fence_after_sync();
       const int row0 = mb * T::TILE_M + int(cta_rank) * 128 + quarter * 32;
+      const int rows = min(32, p.M - row0);  // may be negative
       const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(ab * T::ACC_STEP);
-#pragma unroll 1
-      for (int i = 0; i < T::UNITS / 2; ++i) {
-        // Group 0 begins with the unit that the other accumulator overlaps (the last one of accumulator 0, the
-        // first one of accumulator 1); group 1 has the units between.
-        const int unit = T::UNITS == 2 ? group : (group == 0 ? ((i ^ ab) ? 0 : 3) : 1 + i);
-        const int n0 = nb * BN + unit * 64;
-        uint32_t v[2][32];
-        tmem_ld_32x32(taddr + uint32_t(unit * 64), v[0]);
-        tmem_ld_32x32(taddr + uint32_t(unit * 64 + 32), v[1]);
+      uint32_t v[2][32];
+      tmem_ld_32x32(taddr + uint32_t(unit_of(0) * 64), v[0]);
+      tmem_ld_32x32(taddr + uint32_t(unit_of(0) * 64 + 32), v[1]);
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
         tmem_ld_wait();
         if (i == 0) {
           tc_fence_before_sync();
@@ -396,49 +413,59 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             if constexpr (CG == 2) mbar_arrive_cluster(map_to_cta(smem_u32(acc_go), 0)); else mbar_arrive(acc_go);
           }
         }
-        if (n0 >= p.N) continue;
 #pragma unroll
-        for (int box = 0; box < 64 / BOX_COLS; ++box) {
-          const int c0 = n0 + box * BOX_COLS;
-          uint32_t w[32];
-          mx_finish<EPI>(p, c0, v[box], w);
-          if constexpr (EPI != EPI_F32) mx_finish<EPI>(p, n0 + 32, v[1], w + 16);
-          if (p.tma_store && lane == 0) tma_store_wait_read<0>();  // this warp's previous store has read the buffer
-          __syncwarp();
+        for (int h = 0; h < 2; ++h) {
+          const int n0 = nb * BN + unit_of(i) * 64 + 32 * h;
+          const int c0 = EPI == EPI_F32 ? n0 : n0 - 32 * h, cols = min(BOX_COLS, p.N - c0);  // the box's columns
+          uint32_t w[EPI == EPI_F32 ? 32 : 16];
+          mx_finish<EPI>(p, bias_buf + 64 * i + 32 * h, v[h], w);
+          // the registers are free: the next unit's values may come
+          if (i + 1 < MINE) tmem_ld_32x32(taddr + uint32_t(unit_of(i + 1) * 64 + 32 * h), v[h]);
+          if (EPI == EPI_F32 || h == 0) {
+            if (p.tma_store && lane == 0) tma_store_wait_read<0>();  // this warp's previous store has read the box
+            __syncwarp();
+          }
+          const int chunk0 = EPI == EPI_F32 ? 0 : h * HALF_CHUNKS;
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-            *reinterpret_cast<uint4*>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) =
-                make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+          for (int u = 0; u < HALF_CHUNKS; ++u)
+            *reinterpret_cast<uint4*>(box_at(lane, 16 * (chunk0 + u))) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+          if (EPI != EPI_F32 && h == 0) continue;
           if (p.tma_store) {
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0 && row0 < p.M && c0 < p.N) {
-              tma_store_2d(&tmap_c, buf, c0, row0);
+            if (lane == 0 && rows > 0 && cols > 0) {
+              tma_store_2d(&tmap_c, box, c0, row0);
               tma_store_commit();
             }
           } else {
-            // C or its rows are not 16-byte aligned: the warp writes the box row by row, consecutive lanes
-            // consecutive words; a row of 16-bit values that begins in the middle of a word gives its first value
-            // on its own.  (Each lane storing its own row, element by element: 230 us for 951 x 23085, this LLL.)
+            // C or its rows are not 16-byte aligned: the warp writes the box row by row, consecutive lanes consecutive
+            // words; a row of 16-bit values that begins in the middle of a word gives its first value on its own.
+            // (Each lane storing its own row, element by element: 230 us for 951 x 23085 with K = 68, this 54.)
             __syncwarp();
-            const int rows = min(32, p.M - row0), cols = min(BOX_COLS, p.N - c0);
-            char* crow = static_cast<char*>(p.C) + (int64_t(row0) * p.ldc + c0) * OUT_BYTES;
-            for (int r = 0; r < rows; ++r, crow += p.ldc * OUT_BYTES) {
-              const uint8_t* line = buf + r * 128;
-              auto at = [&](int byte) { return line + ((((byte >> 4) ^ r) & 7) << 4) + (byte & 15); };
-              if constexpr (EPI == EPI_F32) {
-                if (lane < cols) reinterpret_cast<uint32_t*>(crow)[lane] = *reinterpret_cast<const uint32_t*>(at(4 * lane));
-              } else {
-                const int odd = int(reinterpret_cast<uintptr_t>(crow) >> 1) & 1, e = odd + 2 * lane;
-                uint16_t* c16 = reinterpret_cast<uint16_t*>(crow);
-                const uint32_t lo = e < 64 ? *reinterpret_cast<const uint16_t*>(at(2 * e)) : 0u;
-                const uint32_t hi = e + 1 < 64 ? *reinterpret_cast<const uint16_t*>(at(2 * e + 2)) : 0u;
-                if (e + 1 < cols) *reinterpret_cast<uint32_t*>(c16 + e) = lo | (hi << 16);
-                else if (e < cols) c16[e] = uint16_t(lo);
-                if (odd && lane == 0) c16[0] = *reinterpret_cast<const uint16_t*>(at(0));
+            char* corner = static_cast<char*>(p.C) + (int64_t(row0) * p.ldc + c0) * OUT_BYTES;
+            if constexpr (EPI == EPI_F32) {
+#pragma unroll 8
+              for (int r = 0; r < 32; ++r)
+                if (r < rows && lane < cols)
+                  reinterpret_cast<uint32_t*>(corner + int64_t(r) * p.ldc * 4)[lane] = *reinterpret_cast<const uint32_t*>(box_at(r, 4 * lane));
+            } else {
+#pragma unroll 4
+              for (int r = 0; r < rows; ++r) {
+                uint16_t* c16 = reinterpret_cast<uint16_t*>(corner + int64_t(r) * p.ldc * 2);
+                if ((reinterpret_cast<uintptr_t>(c16) & 2) == 0) {
+                  const uint32_t both = *reinterpret_cast<const uint32_t*>(box_at(r, 4 * lane));
+                  if (2 * lane + 1 < cols) reinterpret_cast<uint32_t*>(c16)[lane] = both;
+                  else if (2 * lane < cols) c16[2 * lane] = uint16_t(both);
+                } else {
+                  const int e = 2 * lane + 1;
+                  const uint32_t lo = *reinterpret_cast<const uint16_t*>(box_at(r, 2 * e));
+                  const uint32_t hi = *reinterpret_cast<const uint16_t*>(box_at(r, 2 * min(e + 1, 63)));
+                  if (e + 1 < cols) *reinterpret_cast<uint32_t*>(c16 + e) = lo | (hi << 16);
+                  else if (e < cols) c16[e] = uint16_t(lo);
+                  if (lane == 0 && cols > 0) c16[0] = *reinterpret_cast<const uint16_t*>(box_at(r, 0));
+                }
               }
             }
-            __syncwarp();
           }
         }
       }
