@@ -1,4 +1,4 @@
-"""Builds ``libb200gemm.so`` in-tree with nvcc for sm_100a.
+"""Builds ``libb200gemm.so`` in-tree with nvcc for sm_100a, and the torch binding of its MXFP4 entry points.
 
     python -m cudaintro_b200.build            # build if sources are newer than the library
     python -m cudaintro_b200.build --force
@@ -7,13 +7,15 @@
                                               # kernel accounts for its waits (see cudaintro_b200/timeline.py)
 
 The library is a plain C-ABI shared object (see ``include/b200gemm.h``); nothing in it links
-against Python or torch.  Objects are compiled in parallel, one nvcc per source file.
+against Python or torch.  Objects are compiled in parallel, one nvcc per source file.  The binding,
+``_torch_binding.so``, is a CPython module of its own (``csrc/torch_binding.cpp``) that links against both.
 """
 from __future__ import annotations
 
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -51,7 +53,39 @@ def needs_build() -> bool:
     return newest > _mtime(LIB)
 
 
+BINDING = os.path.join(PKG, "_torch_binding.so")
+BINDING_SOURCE = os.path.join(CSRC, "torch_binding.cpp")
+
+
+def build_binding(force: bool = False) -> str:
+    """Compile the torch binding if it is older than its source or the public header."""
+    newest = max(_mtime(BINDING_SOURCE), _mtime(os.path.join(ROOT, "include", "b200gemm.h")))
+    if not force and _mtime(BINDING) > newest:
+        return BINDING
+    import torch
+
+    base = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", os.path.join(ROOT, "include"), "-isystem", sysconfig.get_paths()["include"],
+           "-isystem", os.path.join(cuda, "include"), "-isystem", os.path.join(base, "include"),
+           "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"), BINDING_SOURCE, "-o", BINDING,
+           "-L", PKG, "-lb200gemm", "-Wl,-rpath,$ORIGIN", "-L", os.path.join(base, "lib"),
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {BINDING_SOURCE}:\n{res.stdout}\n{res.stderr}")
+    return BINDING
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    """Compile the library and its torch binding if needed and return the library's path."""
+    build_library(force, verbose)
+    build_binding(force)
+    return LIB
+
+
+def build_library(force: bool = False, verbose: bool = False) -> str:
     """Compile the library if needed and return its path."""
     if not force and not needs_build():
         return LIB

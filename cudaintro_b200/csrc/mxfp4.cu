@@ -22,11 +22,13 @@ __device__ __forceinline__ T from_f32(float v) {
   else return __float2bfloat16_rn(v);
 }
 
-// Lets the next kernel in the stream (the product that takes what is quantised here) begin its set-up; it waits for this
-// one's end before it reads.  These kernels themselves are launched plainly: as many small CTAs that were let in early
-// would crowd on the SMs that the kernel before leaves first (a layer of 2048 x 4096 -> 11008 called in a row: 57 us, 49
-// plainly).
-__device__ __forceinline__ void mx_let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Set-up of a kernel in a stream: wait for the one before it, and let the next one (the product that takes what is
+// quantised here) begin its own.  Nothing these kernels read is declared read-only for their lifetime (no __ldg, no
+// __restrict__): the compiler may move such loads up past this wait.
+__device__ __forceinline__ void mx_follow_stream() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 
 // A warp's copy of `n` (at most 512) neighbours that are aligned to their element size only, into aligned shared memory;
 // zeros up to 512.  16-bit elements are read as aligned words, the first element on its own where the address asks
@@ -80,7 +82,7 @@ mx_quantize_rows_kernel(const T* x, uint8_t* q, uint8_t* scale, int64_t R,
   const int64_t row_bytes = mx_row_bytes(C);
   const bool live = row < R;
   const int end = min(words, (int(blockIdx.y) + 1) * kRowChunk);
-  mx_let_next_begin();
+  mx_follow_stream();
   for (int w0 = int(blockIdx.y) * kRowChunk; w0 < end; w0 += 4 * UNROLL) {
     Sixteen<T> raw[UNROLL];
 #pragma unroll
@@ -130,7 +132,7 @@ mx_quantize_cols_kernel(const T* x, uint8_t* q, uint8_t* scale, int64_t R,
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row_bytes = mx_row_bytes(R);
   const int64_t c = int64_t(blockIdx.x) * kColTileC + 2 * lane;
-  mx_let_next_begin();
+  mx_follow_stream();
   for (int64_t k0 = int64_t(blockIdx.y) * kColTileK; k0 < int64_t(words) * 128; k0 += int64_t(gridDim.y) * kColTileK) {
     const int64_t r0 = k0 + warp * 32;
     const T* src = x + r0 * ldx + c;
@@ -223,7 +225,7 @@ mx_dequantize_kernel(const uint8_t* q, const uint8_t* scale, T* x, int64_t rows,
   const uint8_t* sr = scale + mx_scale_offset(row, 0, words);
   T* xr = x + row * ldx;
   const int64_t end = min(K, (int64_t(blockIdx.y) + 1) * kDeqChunk);
-  mx_let_next_begin();
+  mx_follow_stream();
   for (int64_t first = int64_t(blockIdx.y) * kDeqChunk; first < end; first += 32 * N * UNROLL) {
     uint32_t codes[UNROLL], byte[UNROLL];
 #pragma unroll
@@ -280,6 +282,26 @@ mx_dequantize_kernel(const uint8_t* q, const uint8_t* scale, T* x, int64_t rows,
   }
 }
 
+// A grid that fills the GPU is launched so that its CTAs may take their places before the kernel ahead of it in the stream
+// has ended (11008 x 4096 back to bf16, called in a row: 20.3 us, 22.5 plainly).  A smaller one is not: all of it would crowd
+// on the SMs that the kernel ahead leaves first (a layer of 2048 x 4096 -> 11008, whose quantiser has 256 CTAs, called in a
+// row: 57 us, 49 plainly).
+template <typename... Args>
+int launch_in_stream(void (*kernel)(Args...), dim3 grid, cudaStream_t stream, std::decay_t<Args>... args) {
+  constexpr int64_t kFull = 148 * 8;  // CTAs of 256 threads that the GPU holds
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kMxThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent_launch_enabled() && int64_t(grid.x) * grid.y >= kFull ? 1 : 0;
+  B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return B200_OK;
+}
+
 template <typename T>
 int quantize_t(const T* x, uint8_t* q, uint8_t* scale, int64_t R, int64_t C, int64_t ldx, int along, cudaStream_t stream) {
   if (along == 0) {
@@ -287,18 +309,14 @@ int quantize_t(const T* x, uint8_t* q, uint8_t* scale, int64_t R, int64_t C, int
     if (chunks > 65535) return fail(B200_ERR_TOO_LARGE, "quantize_mxfp4: rows longer than %lld", 65535LL * kRowChunk * 128);
     const dim3 grid(unsigned(padded / (kMxThreads / 32)), unsigned(chunks));
     const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * int64_t(sizeof(T)) % 16 == 0;
-    (vec ? mx_quantize_rows_kernel<T, true> : mx_quantize_rows_kernel<T, false>)<<<grid, kMxThreads, 0, stream>>>(
-        x, q, scale, R, C, ldx, int(words), padded);
-    B200_CUDA_TRY(cudaGetLastError());
-    return B200_OK;
+    return launch_in_stream(vec ? mx_quantize_rows_kernel<T, true> : mx_quantize_rows_kernel<T, false>, grid, stream, x, q,
+                            scale, R, C, ldx, int(words), padded);
   }
   const int64_t words = (R + 127) / 128, padded = (C + 127) / 128 * 128, tall = (words * 128 + kColTileK - 1) / kColTileK;
   const dim3 grid(unsigned(padded / kColTileC), unsigned(tall < 65535 ? tall : 65535));
   const bool vec = reinterpret_cast<uintptr_t>(x) % (2 * sizeof(T)) == 0 && ldx % 2 == 0;
-  (vec ? mx_quantize_cols_kernel<T, true> : mx_quantize_cols_kernel<T, false>)<<<grid, kMxThreads, 0, stream>>>(
-      x, q, scale, R, C, ldx, int(words));
-  B200_CUDA_TRY(cudaGetLastError());
-  return B200_OK;
+  return launch_in_stream(vec ? mx_quantize_cols_kernel<T, true> : mx_quantize_cols_kernel<T, false>, grid, stream, x, q,
+                          scale, R, C, ldx, int(words));
 }
 
 template <typename T>
@@ -307,10 +325,8 @@ int dequantize_t(const uint8_t* q, const uint8_t* scale, T* x, int64_t rows, int
   if (chunks > 65535) return fail(B200_ERR_TOO_LARGE, "dequantize_mxfp4: rows longer than %lld", 65535LL * kDeqChunk);
   const dim3 grid(unsigned((rows + kMxThreads / 32 - 1) / (kMxThreads / 32)), unsigned(chunks));
   const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * int64_t(sizeof(T)) % 16 == 0;
-  (vec ? mx_dequantize_kernel<T, true> : mx_dequantize_kernel<T, false>)<<<grid, kMxThreads, 0, stream>>>(
-      q, scale, x, rows, K, ldx, int(words));
-  B200_CUDA_TRY(cudaGetLastError());
-  return B200_OK;
+  return launch_in_stream(vec ? mx_dequantize_kernel<T, true> : mx_dequantize_kernel<T, false>, grid, stream, q, scale, x,
+                          rows, K, ldx, int(words));
 }
 
 bool float_dtype(int dtype) { return dtype == B200_F16 || dtype == B200_BF16 || dtype == B200_F32; }
