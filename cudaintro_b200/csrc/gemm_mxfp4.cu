@@ -27,6 +27,7 @@
 #include <cuda_fp16.h>
 
 #include <cstring>
+#include <utility>
 
 #include "internal.h"
 #include "mxfp4.cuh"
@@ -438,9 +439,11 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
               tma_store_commit();
             }
           } else {
-            // C or its rows are not 16-byte aligned: the warp writes the box row by row, consecutive lanes consecutive
-            // words; a row of 16-bit values that begins in the middle of a word gives its first value on its own.
-            // (Each lane storing its own row, element by element: 230 us for 951 x 23085 with K = 68, this 54.)
+            // C or its rows are not 16-byte aligned.  fp32: a row of the box at a time, consecutive lanes consecutive
+            // words.  16 bits: four rows at a time, eight lanes a row.  Where a row begins s elements after a 16-byte
+            // boundary, lanes 1..7 write the seven whole chunks of 16 bytes that it covers, put together from five words of
+            // the box, and the eight elements before and after those go one to a lane.  (Each lane storing its own row,
+            // element by element: 230 us for 951 x 23085 with K = 68; a row at a time in words: 54; this 30.)
             __syncwarp();
             char* corner = static_cast<char*>(p.C) + (int64_t(row0) * p.ldc + c0) * OUT_BYTES;
             if constexpr (EPI == EPI_F32) {
@@ -449,20 +452,31 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                 if (r < rows && lane < cols)
                   reinterpret_cast<uint32_t*>(corner + int64_t(r) * p.ldc * 4)[lane] = *reinterpret_cast<const uint32_t*>(box_at(r, 4 * lane));
             } else {
-#pragma unroll 4
-              for (int r = 0; r < rows; ++r) {
+#pragma unroll 2
+              for (int j = 0; j < 8; ++j) {
+                const int r = 4 * j + (lane >> 3), u = lane & 7;
                 uint16_t* c16 = reinterpret_cast<uint16_t*>(corner + int64_t(r) * p.ldc * 2);
-                if ((reinterpret_cast<uintptr_t>(c16) & 2) == 0) {
-                  const uint32_t both = *reinterpret_cast<const uint32_t*>(box_at(r, 4 * lane));
-                  if (2 * lane + 1 < cols) reinterpret_cast<uint32_t*>(c16)[lane] = both;
-                  else if (2 * lane < cols) c16[2 * lane] = uint16_t(both);
-                } else {
-                  const int e = 2 * lane + 1;
-                  const uint32_t lo = *reinterpret_cast<const uint16_t*>(box_at(r, 2 * e));
-                  const uint32_t hi = *reinterpret_cast<const uint16_t*>(box_at(r, 2 * min(e + 1, 63)));
-                  if (e + 1 < cols) *reinterpret_cast<uint32_t*>(c16 + e) = lo | (hi << 16);
-                  else if (e < cols) c16[e] = uint16_t(lo);
-                  if (lane == 0 && cols > 0) c16[0] = *reinterpret_cast<const uint16_t*>(box_at(r, 0));
+                const int s = int(reinterpret_cast<uintptr_t>(c16) & 15) >> 1;
+                const int e = 8 * u - s;  // lanes 1..7: first element of the chunk
+                uint32_t words[5];
+#pragma unroll
+                for (int k = 0; k < 5; ++k)
+                  words[k] = *reinterpret_cast<const uint32_t*>(box_at(r, min(max(2 * (e & ~1), 0) + 4 * k, 124)));
+                if (r < rows) {
+                  if (u > 0) {
+                    uint32_t out[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) out[k] = s & 1 ? __funnelshift_r(words[k], words[k + 1], 16) : words[k];
+                    if (e + 8 <= cols) {
+                      *reinterpret_cast<uint4*>(c16 + e) = make_uint4(out[0], out[1], out[2], out[3]);
+                    } else {
+#pragma unroll
+                      for (int k = 0; k < 8; ++k)
+                        if (e + k < cols) c16[e + k] = uint16_t(out[k >> 1] >> ((k & 1) * 16));
+                    }
+                  }
+                  const int single = u < 8 - s ? u : 56 + u;
+                  if (single < cols) c16[single] = *reinterpret_cast<const uint16_t*>(box_at(r, 2 * single));
                 }
               }
             }
@@ -498,11 +512,13 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 // S CTAs, one range of K each, so that every SM streams; the partial sums meet through distributed shared
 // memory: each CTA of the cluster finishes 128 / S features, adding the ranges in K order.
 //
-// SRC = 1, 2, 3: the tokens arrive as fp32, fp16 or bf16 rows and six warps quantise this CTA's range of them into
+// SRC = 1, 2, 3: the tokens arrive as fp32, fp16 or bf16 rows and fourteen warps quantise this CTA's range of them into
 // shared memory, in the order the MMA reads, while the weights are on their way: one launch for a layer.
 // SRC = 0: they arrive packed and travel through the ring with the weights.
 //
-// Warp 0 issues the loads, warp 1 the scale copies and MMAs, warps 2-7 quantise, all take part in the tail.  The scale
+// A product of few COLUMNS of C (few rows of B) is the same with the operands in each other's place.
+//
+// Warp 0 issues the loads, warp 1 the scale copies and MMAs, the others quantise, all take part in the tail.  The scale
 // buffers in tensor memory are those of the ring's stages, so a buffer is rewritten only after the stage's MMAs.
 
 enum { SRC_PACKED = 0, SRC_F32 = 1, SRC_F16 = 2, SRC_BF16 = 3 };
@@ -539,6 +555,7 @@ struct MxSkinnyArgs {
   int x_vec;           // rows of X are 16-byte aligned
   const float* bias;
   int relu;
+  int swapped;         // the two operands have changed places: lanes are rows of C, columns its columns
   unsigned long long wait_budget_ns;
   int lose_kb;
 };
@@ -551,8 +568,14 @@ __device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
 
+// Output of token `m`, feature `n`.
 template <int EPI>
 __device__ __forceinline__ void sk_store(const MxSkinnyArgs& p, int m, int n, float y) {
+  if (p.swapped) {
+    const int t = m;
+    m = n;
+    n = t;
+  }
   if (p.bias != nullptr) y += p.bias[n];
   if (p.relu) y = fmaxf(0.0f, y);
   const int64_t at = int64_t(m) * p.ldc + n;
@@ -927,7 +950,7 @@ SkinnyPlan plan_skinny(const MxGemm& g, bool packed, int sms) {
 }
 
 template <int SRC, int EPI>
-int launch_skinny(const MxGemm& g, const SkinnyPlan& plan, cudaStream_t stream) {
+int launch_skinny(const MxGemm& g, const SkinnyPlan& plan, cudaStream_t stream, bool swapped = false) {
   auto kernel = gemm_mx_skinny_kernel<SRC, EPI>;
   static thread_local int last_dev = -1;
   int dev = 0;
@@ -951,6 +974,7 @@ int launch_skinny(const MxGemm& g, const SkinnyPlan& plan, cudaStream_t stream) 
   p.stages = plan.stages;
   p.scale_col = plan.tokens;
   p.tmem_cols = plan.tmem_cols;
+  p.swapped = swapped;
   p.bias = g.tail.bias;
   p.relu = g.tail.flags & B200_LINEAR_RELU;
   wait_test_settings(&p.lose_kb, &p.wait_budget_ns);
@@ -1010,6 +1034,14 @@ int launch_epi(const MxGemm& g, cudaStream_t stream) {
     const SkinnyPlan plan = plan_skinny(g, true, sms);
     if (plan.splits && (g.M <= kSkRows || (plan.splits >= 4 && g.K >= kSkLongK)))
       return launch_skinny<SRC_PACKED, EPI>(g, plan, stream);
+  }
+  if (g.N <= kSkRows && g.M > g.N) {
+    MxGemm t = g;
+    std::swap(t.A, t.B);
+    std::swap(t.a_scale, t.b_scale);
+    std::swap(t.M, t.N);
+    const SkinnyPlan plan = plan_skinny(t, true, sms);
+    if (plan.splits) return launch_skinny<SRC_PACKED, EPI>(t, plan, stream, true);
   }
   // CTA pairs once they give every pair of SMs a tile.
   const int64_t pair_tiles = ((g.M + 255) / 256) * ((g.N + 255) / 256);

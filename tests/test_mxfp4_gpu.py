@@ -114,7 +114,8 @@ def test_dequantise_reads_every_code_and_scale(cb, device, dtype):
 PRODUCTS = [(1, 1, 1), (1, 8, 32), (3, 5, 31), (2, 129, 33), (1, 1000, 4096), (8, 264, 2048), (16, 1000, 7200), (17, 640, 96),
             (32, 4096, 512), (33, 70, 4100), (64, 200, 1024), (65, 384, 640), (100, 136, 784), (128, 128, 128), (129, 127, 65),
             (192, 513, 1000), (256, 192, 96), (257, 512, 784), (256, 256, 256), (512, 520, 7264), (513, 1100, 260),
-            (1000, 1544, 2056), (2304, 2176, 320), (4096, 1024, 64)]
+            (1000, 1544, 2056), (2304, 2176, 320), (4096, 1024, 64), (391, 1037, 160), (515, 333, 96), (2305, 2179, 70), (700, 8, 96),
+            (1000, 32, 2056), (4100, 1, 1000), (130, 17, 7000), (33, 32, 4096)]
 
 
 def exact_case(device, M, N, K):
