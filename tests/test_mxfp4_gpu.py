@@ -348,3 +348,140 @@ def test_wrappers_refuse_what_does_not_belong_together(cb, device):
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+# ------------------------------------------------------------------ what the documentation allows besides
+
+
+def test_results_go_into_given_tensors(cb, device):
+    (a, sa), (b, sb), want = exact_case(device, 70, 264, 320)
+    out = torch.full((70, 264), float("nan"), device=device)
+    assert cb.gemm_mxfp4(a, sa, b, sb, torch.float32, out=out) is not None and same(out, want)
+    x, (w, sw), bias, sums = layer_case(device, torch.float16, 9, 320, 72)
+    y = torch.empty((9, 72), device=device, dtype=torch.float16)
+    cb.linear_mxfp4(x, w, sw, bias=bias, relu=False, out=y)
+    assert same(y, (sums + bias.double()).half())
+    q, s = cb.quantize_mxfp4(x=x, along=0)
+    back = torch.empty((9, 320), device=device, dtype=torch.bfloat16)
+    cb.dequantize_mxfp4(q, s, K=320, dtype=torch.bfloat16, out=back)
+    assert same(back, plain.values(*plain.unpack(q, s)).bfloat16())
+
+
+@pytest.mark.parametrize("n", [5, 130, 700])
+def test_one_matrix_as_both_operands(cb, device, n):
+    """A product of a matrix with itself: the same tensors twice, and a symmetric result to the last bit."""
+    g = generator(device, n)
+    code, byte = plain.random_packed(n, 160, -1, 1, g)
+    q, s = plain.pack(code, byte)
+    got = cb.gemm_mxfp4(q, s, q, s, torch.float32)
+    v = plain.values(code, byte)
+    assert same(got, v @ v.t()) and torch.equal(got, got.t())
+    cb.check_device()
+
+
+def test_garbage_behind_the_matrix_does_not_matter(cb, device):
+    """Packed rows in the middle of a larger buffer whose other bytes are NaN scales and all codes."""
+    from cudaintro_b200 import capi
+
+    for M, N, K in ((3, 130, 96), (150, 40, 160), (300, 300, 256)):
+        (a, sa), (b, sb), want = exact_case(device, M, N, K)
+        held = []
+        for t in (a, sa, b, sb):
+            room = torch.full((t.numel() + 8192,), 255, dtype=torch.uint8, device=device)
+            room[4096 : 4096 + t.numel()] = t.flatten()
+            held.append(room)
+        c = torch.empty((M, N), device=device)
+        p = [r.data_ptr() + 4096 for r in held]
+        assert capi.lib.b200_gemm_mxfp4(capi.F32, *p, c.data_ptr(), M, N, K, 0, torch.cuda.current_stream().cuda_stream) == 0
+        cb.check_device()
+        assert same(c, want)
+
+
+def test_workspace_of_any_allowed_alignment(cb, device):
+    from cudaintro_b200 import capi
+
+    x, (w, sw), bias, sums = layer_case(device, torch.bfloat16, 150, 800, 264)
+    need = capi.lib.b200_linear_mxfp4_workspace(150, 800)
+    assert need > 0
+    for shift in (0, 16, 48, 240):
+        room = torch.full((need + 512,), 255, dtype=torch.uint8, device=device)
+        y = torch.empty((150, 264), dtype=torch.bfloat16, device=device)
+        assert room.data_ptr() % 512 == 0
+        rc = capi.lib.b200_linear_mxfp4(capi.BF16, x.data_ptr(), w.data_ptr(), sw.data_ptr(), bias.data_ptr(), y.data_ptr(), 150, 800,
+                                        264, 0, room.data_ptr() + shift, need, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        cb.check_device()
+        assert same(y, (sums + bias.double()).bfloat16())
+        assert (room[:shift] == 255).all() and (room[shift + need :] == 255).all()
+
+
+def test_layers_longer_than_a_launch_quantises(cb, device):
+    """Rows too long, or too many, for the product to quantise them itself, at the borders of that rule."""
+    for batch, in_f in ((16, 4096), (17, 3872), (64, 1024), (65, 1024), (1, 65536), (1, 65568), (2, 70000)):
+        g = generator(device, batch + in_f)
+        code, byte = plain.random_packed(batch, in_f, 0, 0, g)
+        code[:, 0::32] = 7
+        x = plain.values(code, byte)[:, :in_f].float()
+        w = plain.random_packed(24, in_f, 0, 0, g)
+        w[0][:, 4096:] = 0  # few terms, so that fp32 holds the sums
+        y = cb.linear_mxfp4(x, *plain.pack(*w))
+        cb.check_device()
+        assert same(y, x.double() @ plain.values(*w)[:, :in_f].t())
+
+
+@pytest.mark.parametrize("shape", [(300, 520, 768), (2304, 2304, 768), (40, 300, 768), (8, 264, 4096), (900, 16, 4096)])
+def test_a_lost_arrival_is_reported_and_the_next_call_is_right(cb, device, shape):
+    """Every wait is bounded: with one k-block's loads left out in the first CTA the product gives up after the 50 ms it is
+    given here, says so, and works again.  CTA pairs, single CTAs, and clusters that split K."""
+    import time
+
+    from cudaintro_b200 import capi
+
+    M, N, K = shape
+    (a, sa), (b, sb), want = exact_case(device, M, N, K)
+    assert same(cb.gemm_mxfp4(a, sa, b, sb, torch.float32), want)
+    cb.check_device()
+    try:
+        capi._check(capi.lib.b200_test_lose_arrival(1, 50_000_000))
+        t0 = time.perf_counter()
+        cb.gemm_mxfp4(a, sa, b, sb, torch.float32)
+        with pytest.raises(cb.B200Error) as info:
+            cb.check_device()
+        assert info.value.status == 4 and 0.04 <= time.perf_counter() - t0 < 2.0
+    finally:
+        capi._check(capi.lib.b200_test_lose_arrival(-1, 0))
+    cb.check_device()
+    for _ in range(2):
+        assert same(cb.gemm_mxfp4(a, sa, b, sb, torch.float32), want)
+    cb.check_device()
+
+
+def test_offsets_beyond_32_bits(cb, device):
+    """A matrix of 4.7e9 elements there and back, and a product with 4.4e9 results: first, middle and last rows."""
+    if torch.cuda.mem_get_info(device)[0] < 60e9:
+        pytest.skip("needs 60 GB of free device memory")
+    rows, K = 36000, 131072
+    g = generator(device, 2)
+    x = torch.empty((rows, K), dtype=torch.bfloat16, device=device)
+    picks = [0, 1, 16385, 32768, 35999]
+    x.normal_(generator=g)
+    q, s = cb.quantize_mxfp4(x)
+    back = cb.dequantize_mxfp4(q, s, K, torch.bfloat16)
+    want = plain.values(*plain.quantize(x[picks])).bfloat16()
+    assert same(back[picks], want)
+    del back, q, s
+    # the same memory as columns: K = 36000 down, the last columns' elements lie beyond 2^32
+    q, s = cb.quantize_mxfp4(x, 1)
+    assert tuple(q.shape) == (K, 18000)
+    cols = [0, 65536, K - 1]
+    code, byte = plain.quantize(x[:, cols].t())
+    got = torch.stack([torch.stack([q[c] & 15, q[c] >> 4], -1).flatten() for c in cols])
+    assert torch.equal(got.long(), code)
+    del x, q, s
+    n = 66000
+    a, sa = plain.pack(*plain.random_packed(n, 64, -1, 1, g))
+    c = cb.gemm_mxfp4(a, sa, a, sa)
+    cb.check_device()
+    v = plain.values(*plain.unpack(a, sa))
+    for r in (0, 32769, 65074, n - 1):
+        assert same(c[r], (v @ v[r]).bfloat16())
