@@ -45,7 +45,7 @@ SIGNATURES = {
     "b200_quantize_mxfp4": (_int, [_int, _p, _p, _p, _i64, _i64, _i64, _int, _p]),
     "b200_dequantize_mxfp4": (_int, [_int, _p, _p, _p, _i64, _i64, _i64, _p]),
     "b200_gemm_mxfp4": (_int, [_int, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p]),
-    "b200_linear_mxfp4_workspace": (C.c_size_t, [_i64, _i64]),
+    "b200_linear_mxfp4_workspace": (C.c_size_t, [_i64, _i64, _i64]),
     "b200_linear_mxfp4": (_int, [_int, _p, _p, _p, _p, _p, _i64, _i64, _i64, _int, _p, C.c_size_t, _p]),
     "b200_gemm_host": (_int, [_int, _p, _p, _p, _i64, _i64, _i64, _int]),
     "b200_host_release": (_int, []),

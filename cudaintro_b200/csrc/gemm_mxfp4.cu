@@ -531,11 +531,12 @@ constexpr int kSkMaxPieces = 16;  // pieces of 512 elements in a CTA's range of 
 // rows 14.0 / 19.6, 128 rows 22.4 / 20.0 (32 tiles, four ranges); [1024, 2048], 48 rows 7.4 / 5.9 (eight ranges of one
 // k-block).  So: up to 32 rows always, up to 64 where K is cut in four or more and at least 4096 long.
 constexpr int kSkRows = 32, kSkMaxRows = 64, kSkLongK = 4096;
-// Rows that the kernel quantises itself: 16 rows of 11008 into 4096 features take 12.0 us in one launch (8.5 of them the
-// product's, the quantising is done again by every tile of features), 15 us in two; 32 rows 21 us in one, 15.4 in two.
-// What the quantising costs a CTA goes with rows x its range, so up to 64 short rows are taken too.
-constexpr int kSkFusedRows = 16;
-constexpr int64_t kSkFusedElements = 65536;
+// Rows that the kernel quantises itself, which every tile of features does again, against a quantiser's launch before it.
+// One launch / two, us of a call in a row: 1 row [11008, 4096] 8.9 / 14.4, 16 rows 14.7 / 16.5; 16 rows [4096, 11008] 12.0 /
+// 16.5; 32 rows [4096, 4096] 9.9 / 12.3, [1024, 1024] 8.3 / 10.3; 64 rows [1024, 1024] 11.9 / 8.4; 1 row [28672, 8192], more tiles
+// than SMs, 43.3 / 28.7.  So: up to 16 rows, up to 32 of a limited number of elements, where every tile has an SM.
+constexpr int kSkFusedRows = 16, kSkFusedMaxRows = 32;
+constexpr int64_t kSkFusedElements = 131072, kSkFusedN = 148 * 128;
 constexpr int64_t kSkFusedK = 65536;      // ... and their length: an eighth of it fits in shared memory
 constexpr int kWeightBytes = 128 * 128;     // 128 features x 256 elements
 constexpr int kWeightScales = 2 * kScaleTile;
@@ -1059,8 +1060,8 @@ int launch_mx_gemm(int out_dtype, const MxGemm& g, cudaStream_t stream) {
   }
 }
 
-bool mx_layer_in_one_launch(int64_t rows, int64_t K) {
-  return K <= kSkFusedK && (rows <= kSkFusedRows || (rows <= kSkMaxRows && rows * K <= kSkFusedElements));
+bool mx_layer_in_one_launch(int64_t rows, int64_t K, int64_t N) {
+  return K <= kSkFusedK && N <= kSkFusedN && (rows <= kSkFusedRows || (rows <= kSkFusedMaxRows && rows * K <= kSkFusedElements));
 }
 
 int launch_mx_layer(int dtype, const MxGemm& g, cudaStream_t stream) {

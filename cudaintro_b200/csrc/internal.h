@@ -74,7 +74,7 @@ int encode_tiled_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const
 struct MxGemm;
 int launch_mx_gemm(int out_dtype, const MxGemm& g, cudaStream_t stream);
 // The layer on rows that are not quantised yet, in one launch; for the products that mx_layer_in_one_launch accepts.
-bool mx_layer_in_one_launch(int64_t rows, int64_t K);
+bool mx_layer_in_one_launch(int64_t rows, int64_t K, int64_t N);
 int launch_mx_layer(int dtype, const MxGemm& g, cudaStream_t stream);
 int read_and_clear_mx_status(uint32_t* out);
 

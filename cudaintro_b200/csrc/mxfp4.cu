@@ -434,8 +434,9 @@ extern "C" int b200_gemm_mxfp4(int out_dtype, const void* A, const void* a_scale
   return launch_mx_gemm(out_dtype, g, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" size_t b200_linear_mxfp4_workspace(int64_t batch, int64_t in_features) {
-  if (batch <= 0 || in_features <= 0 || mx_layer_in_one_launch(batch, in_features)) return 0;
+extern "C" size_t b200_linear_mxfp4_workspace(int64_t batch, int64_t in_features, int64_t out_features) {
+  if (batch <= 0 || in_features <= 0 || out_features <= 0) return 0;
+  if (mx_layer_in_one_launch(batch, in_features, out_features)) return 0;
   return b200_mxfp4_scale_bytes(batch, in_features) + size_t(batch) * b200_mxfp4_row_bytes(in_features);
 }
 
@@ -461,7 +462,7 @@ extern "C" int b200_linear_mxfp4(int dtype, const void* X, const void* W, const 
   g.ldc = out_features;
   g.tail.bias = bias;
   g.tail.flags = flags;
-  const size_t need = b200_linear_mxfp4_workspace(batch, in_features);
+  const size_t need = b200_linear_mxfp4_workspace(batch, in_features, out_features);
   if (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16))
     return fail(B200_ERR_BAD_ARGUMENT, "linear_mxfp4: the workspace must be given, 16-byte aligned");
   if (workspace_bytes < need)

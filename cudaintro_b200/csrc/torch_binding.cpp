@@ -247,7 +247,7 @@ PyObject* linear_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject*
   if (relu < 0) return nullptr;
   at::Tensor out, ws;
   if (!result(v[5], batch, out_f, x->scalar_type(), device, &out)) return nullptr;
-  const size_t need = b200_linear_mxfp4_workspace(batch, in_f);
+  const size_t need = b200_linear_mxfp4_workspace(batch, in_f, out_f);
   void* pws = nullptr;
   if (need) {
     ws = at::detail::empty_cuda({int64_t(need)}, at::kByte, device, std::nullopt);

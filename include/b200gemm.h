@@ -317,10 +317,10 @@ int b200_gemm_mxfp4(int out_dtype, const void* A, const void* a_scale, const voi
  * rows.  X [batch, in_features] and Y [batch, out_features] are packed row-major matrices of `dtype` (B200_F32,
  * B200_F16 or B200_BF16); W and w_scale a quantised [out_features, in_features] matrix; bias and flags as in
  * b200_linear (the bias is added to the finished fp32 sum).  workspace: device memory for the quantised X,
- * 16-byte aligned, at least b200_linear_mxfp4_workspace(batch, in_features) bytes; a call uses it until its
+ * 16-byte aligned, at least b200_linear_mxfp4_workspace(...) bytes for the same sizes; a call uses it until its
  * work on `stream` is done, so calls that may overlap need one each.  Where that size is 0 (few rows, which
  * the product quantises itself) it may be NULL. */
-size_t b200_linear_mxfp4_workspace(int64_t batch, int64_t in_features);
+size_t b200_linear_mxfp4_workspace(int64_t batch, int64_t in_features, int64_t out_features);
 int b200_linear_mxfp4(int dtype, const void* X, const void* W, const void* w_scale, const float* bias, void* Y,
                       int64_t batch, int64_t in_features, int64_t out_features, int flags, void* workspace,
                       size_t workspace_bytes, void* stream);

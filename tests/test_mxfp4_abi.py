@@ -17,9 +17,10 @@ def test_sizes_of_packed_arrays(cb):
     assert lib.b200_mxfp4_scale_bytes(129, 128) == 1024 and lib.b200_mxfp4_scale_bytes(129, 129) == 2048
     assert lib.b200_mxfp4_scale_bytes(0, 5) == 0 and lib.b200_mxfp4_scale_bytes(5, -1) == 0
     assert lib.b200_mxfp4_scale_bytes(1 << 30, 1 << 30) == 1 << 55  # no 32-bit wrap
-    assert lib.b200_linear_mxfp4_workspace(200, 784) >= 200 * 400 + 14 * 512
-    assert lib.b200_linear_mxfp4_workspace(1, 4096) == 0 and lib.b200_linear_mxfp4_workspace(1, 1 << 20) > 0
-    assert lib.b200_linear_mxfp4_workspace(0, 784) == 0
+    assert lib.b200_linear_mxfp4_workspace(200, 784, 10) >= 200 * 400 + 14 * 512
+    assert lib.b200_linear_mxfp4_workspace(1, 4096, 11008) == 0 and lib.b200_linear_mxfp4_workspace(1, 1 << 20, 10) > 0
+    assert lib.b200_linear_mxfp4_workspace(1, 4096, 28672) > 0
+    assert lib.b200_linear_mxfp4_workspace(0, 784, 10) == 0
 
 
 def test_plain_form_packs_and_unpacks():
@@ -61,7 +62,7 @@ def test_refusals(cb):
         (gemm, [dict(dtype=i8), dict(a=None), dict(sa=None), dict(b=None), dict(sb=None), dict(c=None), dict(M=0), dict(N=0),
                 dict(K=0), dict(ldc=3)]),
         (linear, [dict(dtype=i8), dict(x=None), dict(w=None), dict(sw=None), dict(y=None), dict(batch=0), dict(i=0), dict(o=0),
-                  dict(flags=4), dict(ws=None), dict(n=0), dict(n=lib.b200_linear_mxfp4_workspace(200, 64) - 1), dict(ws=odd)]),
+                  dict(flags=4), dict(ws=None), dict(n=0), dict(n=lib.b200_linear_mxfp4_workspace(200, 64, 4) - 1), dict(ws=odd)]),
     ):
         for kw in wrong:
             assert call(**kw) == 1, (call.__name__, kw)

@@ -401,7 +401,7 @@ def test_workspace_of_any_allowed_alignment(cb, device):
     from cudaintro_b200 import capi
 
     x, (w, sw), bias, sums = layer_case(device, torch.bfloat16, 150, 800, 264)
-    need = capi.lib.b200_linear_mxfp4_workspace(150, 800)
+    need = capi.lib.b200_linear_mxfp4_workspace(150, 800, 264)
     assert need > 0
     for shift in (0, 16, 48, 240):
         room = torch.full((need + 512,), 255, dtype=torch.uint8, device=device)
@@ -417,7 +417,7 @@ def test_workspace_of_any_allowed_alignment(cb, device):
 
 def test_layers_longer_than_a_launch_quantises(cb, device):
     """Rows too long, or too many, for the product to quantise them itself, at the borders of that rule."""
-    for batch, in_f in ((16, 4096), (17, 3872), (64, 1024), (65, 1024), (1, 65536), (1, 65568), (2, 70000)):
+    for batch, in_f in ((16, 4096), (17, 4096), (17, 7712), (32, 4096), (33, 1024), (64, 1024), (1, 65536), (1, 65568), (2, 70000)):
         g = generator(device, batch + in_f)
         code, byte = plain.random_packed(batch, in_f, 0, 0, g)
         code[:, 0::32] = 7
