@@ -27,6 +27,7 @@
 #include <cuda_fp16.h>
 
 #include <cstring>
+#include <type_traits>
 #include <utility>
 
 #include "internal.h"
@@ -160,6 +161,7 @@ struct MxArgs {
   int relu;
   unsigned long long wait_budget_ns;
   int lose_kb;  // test of the give-up path: k-block of CTA 0's first tile that is never loaded; -1 = none
+  int splits, kb_per_split;  // gemm_mx_split_kernel: CTAs of a cluster = ranges of K, k-blocks of a range
 };
 
 // Groups of group_m tiles of rows; inside a group m runs fastest (a wave of tiles is then a near-square patch).
@@ -526,16 +528,14 @@ constexpr int kSkQuantWarps = 14;
 __host__ __device__ constexpr int sk_threads(int src) { return src == SRC_PACKED ? 256 : 64 + 32 * kSkQuantWarps; }
 constexpr int kSkMaxStages = 12;
 constexpr int kSkMaxPieces = 16;  // pieces of 512 elements in a CTA's range of a token
-// Rows of A the kernel takes.  Measured against the general kernel (128 x 128 tiles), us: [11008, 4096] weights, 1 row
-// 7.2 / 12.8, 16 rows 9.0 / 12.6, 32 rows 10.7 / 12.6, 64 rows 15.7 / 10.3 (86 tiles, two ranges of K); [4096, 11008], 64
-// rows 14.0 / 19.6, 128 rows 22.4 / 20.0 (32 tiles, four ranges); [1024, 2048], 48 rows 7.4 / 5.9 (eight ranges of one
-// k-block).  So: up to 32 rows always, up to 64 where K is cut in four or more and at least 4096 long.
-constexpr int kSkRows = 32, kSkMaxRows = 64, kSkLongK = 4096;
+// Rows of A the kernel takes.  Against the kernels for 128 x 128 tiles, us: [11008, 4096] weights, 1 row 7.2 / 12.8, 16 rows 9.0 /
+// 12.6, 32 rows 10.7 / 12.6, 64 rows 15.7 / 10.3; [4096, 4096], 32 rows 6.9 / 7.2; [4096, 11008], 64 rows 13.6 / 10.2.
+constexpr int kSkRows = 32;
 // Rows that the kernel quantises itself, which every tile of features does again, against a quantiser's launch before it.
 // One launch / two, us of a call in a row: 1 row [11008, 4096] 8.9 / 14.4, 16 rows 14.7 / 16.5; 16 rows [4096, 11008] 12.0 /
 // 16.5; 32 rows [4096, 4096] 9.9 / 12.3, [1024, 1024] 8.3 / 10.3; 64 rows [1024, 1024] 11.9 / 8.4; 1 row [28672, 8192], more tiles
 // than SMs, 43.3 / 28.7.  So: up to 16 rows, up to 32 of a limited number of elements, where every tile has an SM.
-constexpr int kSkFusedRows = 16, kSkFusedMaxRows = 32;
+constexpr int kSkFusedRows = 16;
 constexpr int64_t kSkFusedElements = 131072, kSkFusedN = 148 * 128;
 constexpr int64_t kSkFusedK = 65536;      // ... and their length: an eighth of it fits in shared memory
 constexpr int kWeightBytes = 128 * 128;     // 128 features x 256 elements
@@ -565,6 +565,10 @@ template <int SRC> struct SkSource { using type = float; };
 template <> struct SkSource<SRC_F16> { using type = __half; };
 template <> struct SkSource<SRC_BF16> { using type = __nv_bfloat16; };
 
+__device__ __forceinline__ void st_cluster_v4(uint32_t cluster_addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
 __device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
@@ -813,6 +817,211 @@ gemm_mx_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   }
 }
 
+// ------------------------------------------------------------------------------ few tiles, long K
+//
+// A product with too few 128 x 128 tiles to occupy the GPU runs at the pace of one CTA per tile (a k-block, 34 KB, takes
+// an SM about 0.4 us to pull in).  Here a tile belongs to a cluster of S CTAs, one range of K each.  The partial sums
+// meet through distributed shared memory: the tile's columns are dealt out, 128 / S to a CTA; every epilogue warp sends
+// its 32 rows to the owners, 16 bytes (four columns) a lane, into the slot of its range; after a cluster barrier every
+// CTA adds the slots of its columns in K order and finishes them.
+// Slots: [range][four columns][row][4 floats], so that consecutive lanes (rows) are neighbours on both sides.
+
+struct MxSplit {
+  static constexpr int STAGE_BYTES = MxTile<1, 128>::STAGE_BYTES;
+  static constexpr int EXCHANGE_BYTES = 128 * 128 * 4;
+  static constexpr int STAGES = (kSmemBudget - 2048 - EXCHANGE_BYTES) / STAGE_BYTES;
+  static constexpr int SMEM_BYTES = kSmemBudget;
+  static constexpr int TMEM_COLS = 256;  // 128 of sums, 16 of scales for each stage
+  static_assert(128 + 16 * STAGES <= TMEM_COLS, "tensor memory");
+};
+
+template <int EPI>
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_mx_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                     const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sb, const MxArgs p) {
+  using T = MxTile<1, 128>;
+  constexpr int STAGES = MxSplit::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* exch = smem + STAGES * T::STAGE_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(exch + MxSplit::EXCHANGE_BYTES);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* acc_full = empty_bar + STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int S = p.splits;
+  const uint32_t rank = cluster_cta_rank();
+  const int tile = int(blockIdx.x) / S;
+  const int mb = tile % p.tiles_m, nb = tile / p.tiles_m;
+  const int num_kb = (p.blocks + 7) / 8;
+  const int kb0 = int(rank) * p.kb_per_split;
+  const int kb_count = min(p.kb_per_split, num_kb - kb0);  // never empty
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_b);
+    tma_prefetch_desc(&tmap_sa);
+    tma_prefetch_desc(&tmap_sb);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, MxSplit::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncwarp();
+  cluster_sync_all();  // every CTA of the cluster runs from here on
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ loads
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < kb_count; ++i) {
+      if (!warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_budget_ns)) break;
+      const int kb = kb0 + i;
+      const bool lost = kb == p.lose_kb && blockIdx.x == 0;
+      if (!lost && elect_lane()) {
+        uint8_t* sa = smem + stage * T::STAGE_BYTES;
+        uint8_t* sb = sa + T::A_BYTES;
+        uint8_t* ssa = sb + T::B_BYTES;
+        uint8_t* ssb = ssa + T::SA_BYTES;
+        mbar_arrive_expect_tx(&full_bar[stage], T::STAGE_BYTES);
+        tma_load_2d(sa, &tmap_a, &full_bar[stage], kb * 128, mb * 128);
+        tma_load_2d(sb, &tmap_b, &full_bar[stage], kb * 128, nb * 128);
+        mx_load_3d<1>(ssa, &tmap_sa, smem_u32(&full_bar[stage]), 0, kb * 2, mb);
+        mx_load_3d<1>(ssb, &tmap_sb, smem_u32(&full_bar[stage]), 0, kb * 2, nb);
+      }
+      __syncwarp();
+      if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ scale copies and MMAs
+    constexpr uint32_t idesc0 = mx_instr_desc(128, 128, 0), idesc2 = mx_instr_desc(128, 128, 2);
+    const uint32_t ring = smem_u32(smem);
+    const uint32_t a_desc0 = desc_word(ring), b_desc0 = desc_word(ring + T::A_BYTES);
+    const uint32_t s_desc0 = desc_word(ring + T::A_BYTES + T::B_BYTES);
+    constexpr uint32_t kStageStep = T::STAGE_BYTES >> 4;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < kb_count; ++i) {
+      if (!warp_wait(&full_bar[stage], phase, abort_flag, p.wait_budget_ns)) break;
+      tc_fence_after_sync();
+      // the scale buffers are the stages' own: one is rewritten only after its stage's MMAs
+      const uint32_t sa_tmem = tmem_base + uint32_t(128 + stage * 16), sb_tmem = sa_tmem + 8;
+      const uint32_t a_desc = a_desc0 + uint32_t(stage) * kStageStep, b_desc = b_desc0 + uint32_t(stage) * kStageStep;
+      const uint32_t s_desc = s_desc0 + uint32_t(stage) * kStageStep;
+      const int left = p.blocks - (kb0 + i) * 8;
+      if (elect_lane()) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          mx_copy_scales<1>(sa_tmem + uint32_t(4 * h), s_desc + uint32_t((h * kScaleTile) >> 4));
+          mx_copy_scales<1>(sb_tmem + uint32_t(4 * h), s_desc + uint32_t((T::SA_BYTES + h * kScaleTile) >> 4));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (2 * j < left)
+            mx_umma<1>(tmem_base, a_desc + uint32_t(2 * j), b_desc + uint32_t(2 * j), (j & 1) ? idesc2 : idesc0,
+                       sa_tmem + uint32_t(4 * (j >> 1)), sb_tmem + uint32_t(4 * (j >> 1)), (i | j) != 0 ? 1u : 0u);
+        }
+        umma_commit(&empty_bar[stage]);
+        if (i + 1 == kb_count) umma_commit(acc_full);
+      }
+      __syncwarp();
+      if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+    }
+  }
+  __syncwarp();
+
+  const int own = 128 / S, own_units = own / 4;  // columns a CTA finishes, and those in fours
+  if (warp >= 2) {
+    const int group = (warp - 2) >> 2, quarter = warp & 3;
+    const bool ready = warp_wait(acc_full, 0, abort_flag, p.wait_budget_ns);
+    tc_fence_after_sync();
+    if (ready) {
+      const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(group * 64);
+      uint32_t v[2][32];
+      tmem_ld_32x32(taddr, v[0]);
+      tmem_ld_32x32(taddr + 32, v[1]);
+      tmem_ld_wait();
+      const uint32_t slot = smem_u32(exch) + uint32_t((int(rank) * own_units * 128 + quarter * 32 + lane) * 16);
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        const int c = group * 16 + u, owner = c / own_units;  // the c-th four columns of the tile
+        st_cluster_v4(map_to_cta(slot, uint32_t(owner)) + uint32_t((c - owner * own_units) * 128 * 16), v[u >> 3][4 * (u & 7)],
+                      v[u >> 3][4 * (u & 7) + 1], v[u >> 3][4 * (u & 7) + 2], v[u >> 3][4 * (u & 7) + 3]);
+      }
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();  // every range's sums have arrived, and nobody writes into another CTA after this
+
+  if (*abort_flag == 0u) {
+    // eight columns of a row at a time
+    const int units = own / 8 * 128;
+    for (int i = threadIdx.x; i < units; i += kThreads) {
+      const int row = i & 127, g = i >> 7, m = mb * 128 + row, n = nb * 128 + int(rank) * own + g * 8;
+      if (m >= p.M || n >= p.N) continue;
+      float y[8] = {};
+      for (int r = 0; r < S; ++r) {
+        const float4* slot = reinterpret_cast<const float4*>(exch) + (r * own_units + 2 * g) * 128 + row;
+        const float4 lo = slot[0], hi = slot[128];
+        y[0] += lo.x; y[1] += lo.y; y[2] += lo.z; y[3] += lo.w;
+        y[4] += hi.x; y[5] += hi.y; y[6] += hi.z; y[7] += hi.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (p.bias != nullptr) y[e] += p.bias[min(n + e, p.N - 1)];
+        if (p.relu) y[e] = fmaxf(0.0f, y[e]);
+      }
+      using Out = typename std::conditional<EPI == EPI_F32, float, typename std::conditional<EPI == EPI_F16, __half, __nv_bfloat16>::type>::type;
+      alignas(16) Out out[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (EPI == EPI_F32) out[e] = y[e];
+        else if constexpr (EPI == EPI_F16) out[e] = __float2half_rn(y[e]);
+        else out[e] = __float2bfloat16_rn(y[e]);
+      }
+      Out* dst = static_cast<Out*>(p.C) + int64_t(m) * p.ldc + n;
+      if (p.tma_store && n + 8 <= p.N) {  // 16-byte aligned
+#pragma unroll
+        for (int k = 0; k < int(sizeof(out) / 16); ++k) reinterpret_cast<uint4*>(dst)[k] = reinterpret_cast<const uint4*>(out)[k];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (n + e < p.N) dst[e] = out[e];
+      }
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0) atomicOr(&g_mx_status, 4u);
+    // Give copies and MMAs still in flight time to land before shared and tensor memory go away.
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, MxSplit::TMEM_COLS);
+  }
+}
+
 // ------------------------------------------------------------------------------ host side
 
 // Packed elements as bytes: 128-byte swizzle, zeros outside the matrix.
@@ -1026,15 +1235,78 @@ int device_sms(int* sms) {
   return B200_OK;
 }
 
+// Ranges of K for a product of `tiles` 128 x 128 tiles (1 = do not split).  1 / 2 / 4 / 8 ranges, us: K = 2048, 16 tiles 6.1 /
+// 6.2 / 5.5 / 11.3; K = 4096, 14 tiles 9.2 / 7.3 / 6.1 / 6.6, 32 tiles 9.4 / 7.4 / 7.2 / -, 36 tiles 9.4 / 7.4 / 12.6, 74 tiles 9.6 /
+// 8.0; K = 11008, 14 tiles 19.3 / 11.4 / 8.2 / 7.7, 16 tiles 19.3 / 11.4 / 8.3 / 14.1, 32 tiles 19.6 / 11.7 / 9.3, 74 tiles 20.1 /
+// 13.5.  A cluster has to find its CTAs' SMs inside one group of SMs, so not every SM can be used by clusters of four
+// (seven eighths of them) or eight (three quarters) at once; where a cluster has to wait the time doubles.
+int split_ranges(int64_t tiles, int num_kb, int sms) {
+  auto whole = [&](int s) { return ((num_kb + s - 1) / s) * (s - 1) < num_kb; };  // no range is empty
+  if (num_kb >= 32 && tiles * 8 * 4 <= int64_t(sms) * 3 && whole(8)) return 8;
+  if (num_kb >= 8 && tiles * 4 * 8 <= int64_t(sms) * 7 && whole(4)) return 4;
+  if (num_kb >= 12 && tiles * 2 <= sms && whole(2)) return 2;
+  return 1;
+}
+
+template <int EPI>
+int launch_split(const MxGemm& g, int splits, cudaStream_t stream) {
+  auto kernel = gemm_mx_split_kernel<EPI>;
+  static thread_local int last_dev = -1;  // the shared-memory attribute is per device
+  int dev = 0;
+  B200_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev != last_dev) {
+    B200_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MxSplit::SMEM_BYTES));
+    last_dev = dev;
+  }
+  MxArgs p;
+  memset(&p, 0, sizeof(p));
+  p.C = g.C;
+  p.ldc = g.ldc;
+  p.M = int(g.M);
+  p.N = int(g.N);
+  p.blocks = int((g.K + 31) / 32);
+  p.tiles_m = int((g.M + 127) / 128);
+  p.tiles_n = int((g.N + 127) / 128);
+  p.bias = g.tail.bias;
+  p.relu = g.tail.flags & B200_LINEAR_RELU;
+  p.splits = splits;
+  p.kb_per_split = ((p.blocks + 7) / 8 + splits - 1) / splits;
+  wait_test_settings(&p.lose_kb, &p.wait_budget_ns);
+  const int elem = EPI == EPI_F32 ? 4 : 2;
+  p.tma_store = (g.ldc * elem) % 16 == 0 && reinterpret_cast<uintptr_t>(g.C) % 16 == 0;
+  const int64_t row_bytes = mx_row_bytes(g.K), tiles_k = (g.K + 127) / 128;
+  CUtensorMap ma, mb, msa, msb;
+  int rc = map_elements(&ma, g.A, g.M, row_bytes, 128);
+  if (!rc) rc = map_elements(&mb, g.B, g.N, row_bytes, 128);
+  if (!rc) rc = map_scales(&msa, g.a_scale, g.M, tiles_k, 1);
+  if (!rc) rc = map_scales(&msb, g.b_scale, g.N, tiles_k, 1);
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(p.tiles_m * p.tiles_n * splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = MxSplit::SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(splits);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent_launch_enabled() ? 2 : 1;
+  B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, ma, mb, msa, msb, p));
+  return B200_OK;
+}
+
 template <int EPI>
 int launch_epi(const MxGemm& g, cudaStream_t stream) {
   int sms = 0;
   int rc = device_sms(&sms);
   if (rc) return rc;
-  if (g.M <= kSkMaxRows) {
+  if (g.M <= kSkRows) {
     const SkinnyPlan plan = plan_skinny(g, true, sms);
-    if (plan.splits && (g.M <= kSkRows || (plan.splits >= 4 && g.K >= kSkLongK)))
-      return launch_skinny<SRC_PACKED, EPI>(g, plan, stream);
+    if (plan.splits) return launch_skinny<SRC_PACKED, EPI>(g, plan, stream);
   }
   if (g.N <= kSkRows && g.M > g.N) {
     MxGemm t = g;
@@ -1044,6 +1316,9 @@ int launch_epi(const MxGemm& g, cudaStream_t stream) {
     const SkinnyPlan plan = plan_skinny(t, true, sms);
     if (plan.splits) return launch_skinny<SRC_PACKED, EPI>(t, plan, stream, true);
   }
+  const int64_t tiles = ((g.M + 127) / 128) * ((g.N + 127) / 128);
+  const int splits = split_ranges(tiles, int((g.K + 255) / 256), sms);
+  if (splits > 1) return launch_split<EPI>(g, splits, stream);
   // CTA pairs once they give every pair of SMs a tile.
   const int64_t pair_tiles = ((g.M + 255) / 256) * ((g.N + 255) / 256);
   if (g.M > 128 && pair_tiles >= sms / 2) return launch_tile<2, 256, EPI>(g, sms, stream);
@@ -1061,7 +1336,7 @@ int launch_mx_gemm(int out_dtype, const MxGemm& g, cudaStream_t stream) {
 }
 
 bool mx_layer_in_one_launch(int64_t rows, int64_t K, int64_t N) {
-  return K <= kSkFusedK && N <= kSkFusedN && (rows <= kSkFusedRows || (rows <= kSkFusedMaxRows && rows * K <= kSkFusedElements));
+  return K <= kSkFusedK && N <= kSkFusedN && (rows <= kSkFusedRows || (rows <= kSkRows && rows * K <= kSkFusedElements));
 }
 
 int launch_mx_layer(int dtype, const MxGemm& g, cudaStream_t stream) {

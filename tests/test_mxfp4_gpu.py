@@ -115,7 +115,8 @@ PRODUCTS = [(1, 1, 1), (1, 8, 32), (3, 5, 31), (2, 129, 33), (1, 1000, 4096), (8
             (32, 4096, 512), (33, 70, 4100), (64, 200, 1024), (65, 384, 640), (100, 136, 784), (128, 128, 128), (129, 127, 65),
             (192, 513, 1000), (256, 192, 96), (257, 512, 784), (256, 256, 256), (512, 520, 7264), (513, 1100, 260),
             (1000, 1544, 2056), (2304, 2176, 320), (4096, 1024, 64), (391, 1037, 160), (515, 333, 96), (2305, 2179, 70), (700, 8, 96),
-            (1000, 32, 2056), (4100, 1, 1000), (130, 17, 7000), (33, 32, 4096)]
+            (1000, 32, 2056), (4100, 1, 1000), (130, 17, 7000), (33, 32, 4096), (65, 384, 3000), (300, 500, 4097), (128, 4096, 2816),
+            (200, 131, 7200), (700, 900, 2304), (100, 33, 6000)]
 
 
 def exact_case(device, M, N, K):
@@ -429,7 +430,7 @@ def test_layers_longer_than_a_launch_quantises(cb, device):
         assert same(y, x.double() @ plain.values(*w)[:, :in_f].t())
 
 
-@pytest.mark.parametrize("shape", [(300, 520, 768), (2304, 2304, 768), (40, 300, 768), (8, 264, 4096), (900, 16, 4096)])
+@pytest.mark.parametrize("shape", [(300, 520, 768), (2304, 2304, 768), (40, 300, 768), (8, 264, 4096), (900, 16, 4096), (200, 300, 4096)])
 def test_a_lost_arrival_is_reported_and_the_next_call_is_right(cb, device, shape):
     """Every wait is bounded: with one k-block's loads left out in the first CTA the product gives up after the 50 ms it is
     given here, says so, and works again.  CTA pairs, single CTAs, and clusters that split K."""
