@@ -270,6 +270,82 @@ def case_quantize(R, C, along):
     return run
 
 
+def _mx_packed_bytes(rows, k):
+    return rows * -(-k // 32) * 17
+
+
+def case_mxfp4_gemm(M, N, K):
+    """Product of two packed 4-bit matrices, bf16 out, operands rotated through more than L2.  The peak is four times the
+    bf16 rate, the ratio of the tensor cores' nominal rates."""
+    def run(args, device):
+        import cudaintro_b200 as cb
+        import torch
+
+        copies = max(1, min(8, int(2 * L2_BYTES / (_mx_packed_bytes(M, K) + _mx_packed_bytes(N, K))) + 1))
+        sets = [cb.quantize_mxfp4(_randn((M, K), torch.bfloat16, device, i)) + cb.quantize_mxfp4(_randn((N, K), torch.bfloat16, device, 50 + i))
+                for i in range(copies)]
+        turn = [0]
+
+        def fn():
+            turn[0] = (turn[0] + 1) % copies
+            cb.gemm_mxfp4(*sets[turn[0]])
+
+        med, best = _time(fn, args.reps, args.warmup)
+        cb.check_device()
+        byts = _mx_packed_bytes(M, K) + _mx_packed_bytes(N, K) + 2 * M * N
+        hbm, bf16, src = _peaks()
+        tflops = 2 * M * N * K / (med * 1e-3) / 1e12
+        return {"bound": "tensor", "ms_median": med, "ms_best": best, "achieved": tflops, "unit": "TFLOP/s", "peak": 4 * bf16,
+                "peak_source": f"4 x {src} bf16 GEMM", "frac": tflops / (4 * bf16), "algorithmic_bytes": byts}
+    return run
+
+
+def case_mxfp4_linear(M, K, N):
+    """Layer on 4-bit weights (rotated through more than L2), activations in bf16."""
+    def run(args, device):
+        import cudaintro_b200 as cb
+        import torch
+
+        copies = max(1, min(12, int(2 * L2_BYTES / _mx_packed_bytes(N, K)) + 1))
+        ws = [cb.quantize_mxfp4(_randn((N, K), torch.bfloat16, device, i, 0.02)) for i in range(copies)]
+        x = _randn((M, K), torch.bfloat16, device, 99)
+        turn = [0]
+
+        def fn():
+            turn[0] = (turn[0] + 1) % copies
+            cb.linear_mxfp4(x, *ws[turn[0]])
+
+        med, best = _time(fn, args.reps, args.warmup)
+        cb.check_device()
+        byts = 2 * M * K + _mx_packed_bytes(N, K) + 2 * M * N
+        hbm, _, src = _peaks()
+        return {"bound": "hbm", "ms_median": med, "ms_best": best, "achieved": byts / (med * 1e-3) / 1e9, "unit": "GB/s",
+                "peak": hbm, "peak_source": f"{src} HBM copy", "frac": byts / (med * 1e-3) / 1e9 / hbm, "algorithmic_bytes": byts}
+    return run
+
+
+def case_mxfp4_quantize(R, C, along, back=False):
+    """bf16 to packed 4-bit (along rows or columns), or the way back."""
+    def run(args, device):
+        import cudaintro_b200 as cb
+        import torch
+
+        xs = [_randn((R, C), torch.bfloat16, device, i) for i in range(3)]
+        qs = [cb.quantize_mxfp4(x, along) for x in xs]
+        turn = [0]
+
+        def fn():
+            turn[0] = (turn[0] + 1) % 3
+            cb.dequantize_mxfp4(*qs[turn[0]]) if back else cb.quantize_mxfp4(xs[turn[0]], along)
+
+        med, best = _time(fn, args.reps, args.warmup)
+        byts = 2 * R * C + (_mx_packed_bytes(C, R) if along else _mx_packed_bytes(R, C))
+        hbm, _, src = _peaks()
+        return {"bound": "hbm", "ms_median": med, "ms_best": best, "achieved": byts / (med * 1e-3) / 1e9, "unit": "GB/s",
+                "peak": hbm, "peak_source": f"{src} HBM copy", "frac": byts / (med * 1e-3) / 1e9 / hbm, "algorithmic_bytes": byts}
+    return run
+
+
 CASES = {
     "bf16_8192": case_gemm("bf16", 8192, 8192, 8192),
     "fp16_8192": case_gemm("f16", 8192, 8192, 8192),
@@ -295,6 +371,15 @@ CASES = {
     "fc_20000x784x512_tf32": case_fc(20000, 784, 512, "F32_TF32"),
     "quantize_rows_8192x8192": case_quantize(8192, 8192, 0),
     "quantize_cols_8192x28672": case_quantize(8192, 28672, 1),
+    "mxfp4_8192": case_mxfp4_gemm(8192, 8192, 8192),
+    "mxfp4_4096": case_mxfp4_gemm(4096, 4096, 4096),
+    "mxfp4_8192x28672": case_mxfp4_gemm(8192, 28672, 8192),
+    "mxfp4_linear_m1": case_mxfp4_linear(1, 4096, 11008),
+    "mxfp4_linear_m16": case_mxfp4_linear(16, 11008, 4096),
+    "mxfp4_linear_m2048": case_mxfp4_linear(2048, 4096, 11008),
+    "mxfp4_quantize_rows_8192": case_mxfp4_quantize(8192, 8192, 0),
+    "mxfp4_quantize_cols_4096x11008": case_mxfp4_quantize(4096, 11008, 1),
+    "mxfp4_dequantize_8192": case_mxfp4_quantize(8192, 8192, 0, back=True),
 }
 
 
