@@ -532,8 +532,8 @@ constexpr int kSkMaxPieces = 16;  // pieces of 512 elements in a CTA's range of 
 // 12.6, 32 rows 10.7 / 12.6, 64 rows 15.7 / 10.3; [4096, 4096], 32 rows 6.9 / 7.2; [4096, 11008], 64 rows 13.6 / 10.2.
 constexpr int kSkRows = 32;
 // Rows that the kernel quantises itself, which every tile of features does again, against a quantiser's launch before it.
-// One launch / two, us of a call in a row: 1 row [11008, 4096] 8.9 / 14.4, 16 rows 14.7 / 16.5; 16 rows [4096, 11008] 12.0 /
-// 16.5; 32 rows [4096, 4096] 9.9 / 12.3, [1024, 1024] 8.3 / 10.3; 64 rows [1024, 1024] 11.9 / 8.4; 1 row [28672, 8192], more tiles
+// One launch / two, us of a call in a row: 1 row [11008, 4096] 8.7 / 14.4, 16 rows 13.1 / 16.5; 16 rows [4096, 11008] 12.0 /
+// 16.5; 32 rows [4096, 4096] 9.6 / 12.3, [1024, 1024] 7.5 / 10.3; 64 rows [1024, 1024] 11.9 / 8.4; 1 row [28672, 8192], more tiles
 // than SMs, 43.3 / 28.7.  So: up to 16 rows, up to 32 of a limited number of elements, where every tile has an SM.
 constexpr int kSkFusedRows = 16;
 constexpr int64_t kSkFusedElements = 131072, kSkFusedN = 148 * 128;
@@ -715,53 +715,43 @@ gemm_mx_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     }
   } else if constexpr (SRC != SRC_PACKED) {
     // ------------------------------------------------------------------ tokens -> shared memory
-    // A warp takes 512 elements (a piece, two k-blocks) of a token at a time, sixteen a lane, two lanes a block, with the
-    // loads of UNROLL tokens in flight.  The first piece of all tokens comes first, so that its MMAs can start.
-    constexpr int UNROLL = 2;
+    // A warp takes 512 elements (a piece, two k-blocks) of a token at a time, sixteen a lane, two lanes a block.  The first
+    // piece of all tokens comes first, so that its MMAs can start.  (10 / 14 / 18 warps, us: 1 row [11008, 4096] 8.6 / 8.7 /
+    // 9.1, 16 rows [4096, 11008] 14.5 / 12.3 / 12.4, 32 rows [4096, 4096] 10.4 / 9.6 / 10.0; two pieces at a time in 14: 8.9,
+    // 12.0, 10.0.)
     const X* x = static_cast<const X*>(p.X);
     const int pieces = (kb_count + 1) / 2;
     const int piece_step = kSkQuantWarps / p.M, m_step = kSkQuantWarps - piece_step * p.M;
     int piece_next = (warp - 2) / p.M, m_next = (warp - 2) - piece_next * p.M;
     while (piece_next < pieces) {
-      Sixteen<X> raw[UNROLL];
-      int at_m[UNROLL], at_e[UNROLL];
-#pragma unroll
-      for (int i = 0; i < UNROLL; ++i) {
-        at_m[i] = m_next;
-        at_e[i] = piece_next * 512 + lane * 16;
-        const int64_t k = int64_t(kb0) * 256 + at_e[i];
-        load16(x + int64_t(m_next) * p.K + k, piece_next < pieces ? p.K - k : 0, raw[i], p.x_vec != 0);
-        piece_next += piece_step;
-        m_next += m_step;
-        if (m_next >= p.M) {
-          m_next -= p.M;
-          ++piece_next;
-        }
+      const int piece = piece_next, m = m_next, e = piece * 512 + lane * 16;
+      piece_next += piece_step;
+      m_next += m_step;
+      if (m_next >= p.M) {
+        m_next -= p.M;
+        ++piece_next;
       }
-#pragma unroll
-      for (int i = 0; i < UNROLL; ++i) {
-        const int m = at_m[i], e = at_e[i];
-        uint32_t top = top_of<X, Sixteen<X>::WORDS>(raw[i].w);
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        const uint32_t byte = mx_scale_byte(top);
-        const uint2 codes = encode16(raw[i], byte);
-        uint32_t four = byte << (4 * (lane & 6));
-        four |= __shfl_xor_sync(0xffffffffu, four, 2);
-        four |= __shfl_xor_sync(0xffffffffu, four, 4);
-        const int kb = e >> 8;  // k-block within this CTA's range
-        if (kb < kb_count) {
-          // 128-byte swizzle: 16-byte chunk c of row m lies at chunk c ^ (m % 8)
-          const int in_row = (e & 255) >> 1, chunk = (in_row >> 4) ^ (m & 7);
-          *reinterpret_cast<uint2*>(xq + kb * token_bytes + m * 128 + (chunk << 4) + (in_row & 15)) = codes;
-          if ((lane & 7) == 0)
-            *reinterpret_cast<uint32_t*>(xs + kb * 2 * kScaleTile + ((e >> 7) & 1) * kScaleTile + (m & 31) * 16 + (m >> 5) * 4) = four;
-        }
+      Sixteen<X> raw;
+      const int64_t k = int64_t(kb0) * 256 + e;
+      load16(x + int64_t(m) * p.K + k, p.K - k, raw, p.x_vec != 0);
+      uint32_t top = top_of<X, Sixteen<X>::WORDS>(raw.w);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      const uint32_t byte = mx_scale_byte(top);
+      const uint2 codes = encode16(raw, byte);
+      uint32_t four = byte << (4 * (lane & 6));
+      four |= __shfl_xor_sync(0xffffffffu, four, 2);
+      four |= __shfl_xor_sync(0xffffffffu, four, 4);
+      const int kb = e >> 8;  // k-block within this CTA's range
+      if (kb < kb_count) {
+        // 128-byte swizzle: 16-byte chunk c of row m lies at chunk c ^ (m % 8)
+        const int in_row = (e & 255) >> 1, chunk = (in_row >> 4) ^ (m & 7);
+        *reinterpret_cast<uint2*>(xq + kb * token_bytes + m * 128 + (chunk << 4) + (in_row & 15)) = codes;
+        if ((lane & 7) == 0)
+          *reinterpret_cast<uint32_t*>(xs + kb * 2 * kScaleTile + ((e >> 7) & 1) * kScaleTile + (m & 31) * 16 + (m >> 5) * 4) = four;
       }
       fence_proxy_async_smem();  // the MMAs and scale copies read what was written here
       __syncwarp();
-#pragma unroll
-      for (int i = 0; i < UNROLL; ++i)
-        if (lane == 0 && (at_e[i] >> 9) < pieces) mbar_arrive(&x_ready[at_e[i] >> 9]);
+      if (lane == 0) mbar_arrive(&x_ready[piece]);
     }
   }
   __syncwarp();
