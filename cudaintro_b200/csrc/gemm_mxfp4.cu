@@ -21,8 +21,15 @@
 // used in turn: the buffer of k-block i is rewritten only after the MMAs of k-block i - 2 have completed
 // (their commit is waited for), while those of k-block i - 1 keep the tensor pipe busy.
 //
-// Every wait is bounded; a wait that runs out raises the CTA's abort flag, all roles drain, tensor memory is freed
-// and a status word tells the host that the result is invalid.
+// Bound: what an SM takes in.  A k-block is 35 KB of operands and scales for 512 clocks of MMAs, and an SM pulls about 84 GB/s
+// out of L2 whatever the clock, 0.42 us a k-block: 8192^3 to bf16 in 187 us in short bursts (5.9 PFLOP/s; without the loads of
+// B 174 us, with half the MMAs 166 us), 220 us under the power cap.  Three, four and five ring stages: 239, 205, 195 us with
+// the clocks read inside; rows per tile-order group 1024 / 2048 / 4096 / 8192 at 8192 x 28672 x 8192, run for seconds, 830 / 799
+// / 769 / 769 us.  Scales written to tensor memory by four warps (tcgen05.st) instead of copied: 437 us.
+//
+// Below it in this file: the kernel for few rows (or columns), the one that splits K for few tiles, and the rules that
+// choose.  Every wait is bounded; a wait that runs out raises the CTA's abort flag, all roles drain, tensor memory is
+// freed and a status word tells the host that the result is invalid.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -37,7 +44,7 @@
 namespace b200 {
 namespace {
 
-__device__ uint32_t g_mx_status = 0;  // bit 0: a bounded wait ran out somewhere
+__device__ uint32_t g_mx_status = 0;  // a bounded wait ran out: 1 = gemm_mx, 2 = gemm_mx_skinny, 4 = gemm_mx_split
 
 constexpr int kSmemBudget = 227 * 1024;
 constexpr int kEpiWarps = 8;
@@ -508,7 +515,7 @@ gemm_mx_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 
 // ------------------------------------------------------------------------------ few rows of A
 //
-// A product of at most 128 rows of A streams B (the weights) and computes little.  Here the weights are the 128-row
+// A product of at most 32 rows of A streams B (the weights) and computes little.  Here the weights are the 128-row
 // operand of the MMA and the rows of A ("tokens", padded to 16) its N dimension, so no instruction is spent on rows
 // that do not exist, and an accumulator lane is one output feature.  A tile of 128 features is shared by a cluster of
 // S CTAs, one range of K each, so that every SM streams; the partial sums meet through distributed shared

@@ -1,7 +1,11 @@
-// Microscaled 4-bit floating point (MXFP4): quantisation, dequantisation and the products of 4-bit
-// matrices.  The format is that of the Open Compute Project's microscaling specification: 32
-// neighbours along K share one power of two, an element is a sign, two bits of exponent and one of
-// mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6).  Declarations and layouts: include/b200gemm.h.
+// Microscaled 4-bit floating point (MXFP4): quantisation, dequantisation, and the C entry points of the
+// operators (the products' kernels are in gemm_mxfp4.cu).  The format is that of the Open Compute Project's
+// microscaling specification: 32 neighbours along K share one power of two, an element is a sign, two bits of
+// exponent and one of mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6).  Declarations and layouts: include/b200gemm.h.
+//
+// Bound: HBM.  A 16-bit element is read once and 17/32 of a byte written (or the reverse).  Measured, inputs rotated
+// through more than L2: 8192 x 8192 bf16 along rows 29.5 us = 5.75 TB/s (0.88 of the measured copy), fp32 53.5 us =
+// 5.7 TB/s, 4096 x 11008 fp16 along columns 21.9 us = 5.2 TB/s, 11008 x 4096 back to bf16 20.3 us = 5.6 TB/s.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
