@@ -78,6 +78,19 @@ def test_quantise_borders_and_special_values(cb, device, along):
     assert same(back, plain.values(*plain.quantize(x.t() if along else x)).float())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("along", [0, 1])
+def test_quantise_every_16_bit_value(cb, device, along, dtype):
+    """All bit patterns, in order (blocks of one sign and exponent) and shuffled: subnormals, infinities and NaN too."""
+    bits = torch.arange(-32768, 32768, device=device).to(torch.int16)
+    shuffled = bits[torch.randperm(65536, device=device, generator=generator(device, 4))]
+    for b in (bits, shuffled):
+        x = b.view(dtype).reshape(256, 256)
+        check_quantised(cb, x.t().contiguous() if along else x, along)
+    finite = torch.where(torch.isfinite(x), x, torch.zeros_like(x))
+    check_quantised(cb, finite, along)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("along", [0, 1])
 def test_quantise_takes_strided_and_unaligned_rows(cb, device, along, dtype):
@@ -200,7 +213,7 @@ def layer_case(device, dtype, batch, in_f, out_f):
 
 
 LAYERS = [(1, 32, 8), (1, 4096, 1032), (2, 784, 512), (7, 2048, 1024), (16, 4104, 520), (33, 1000, 264), (100, 2048, 1024),
-          (128, 96, 256), (257, 784, 512), (520, 1032, 264)]
+          (128, 96, 256), (257, 784, 512), (520, 1032, 264), (3, 96, 18944), (1, 64, 19000), (32, 4096, 136)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -486,3 +499,51 @@ def test_offsets_beyond_32_bits(cb, device):
     v = plain.values(*plain.unpack(a, sa))
     for r in (0, 32769, 65074, n - 1):
         assert same(c[r], (v @ v[r]).bfloat16())
+
+
+def test_plain_launches_give_the_same(cb, device):
+    """Without programmatic stream serialisation."""
+    from cudaintro_b200 import capi
+
+    def everything():
+        out = []
+        for shape in ((8, 264, 2048), (300, 520, 4096), (2304, 2304, 256)):
+            (a, sa), (b, sb), want = exact_case(device, *shape)
+            got = cb.gemm_mxfp4(a, sa, b, sb, torch.float32)
+            assert same(got, want)
+            out += [got, *cb.quantize_mxfp4(got), cb.linear_mxfp4(got, *cb.quantize_mxfp4(got))]
+        return out
+
+    first = everything()
+    try:
+        capi.lib.b200_set_dependent_launch(0)
+        second = everything()
+    finally:
+        capi.lib.b200_set_dependent_launch(1)
+    cb.check_device()
+    assert all(torch.equal(x, y) for x, y in zip(first, second))
+
+
+def test_host_threads_at_once(cb, device):
+    """Four host threads, a stream and a shape each, the same thread-local and shared state underneath."""
+    import threading
+
+    shapes = [(1, 2048, 1024), (20, 1024, 520), (130, 2048, 264), (300, 4096, 520)]
+    cases = [layer_case(device, torch.bfloat16, *s) for s in shapes]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(x, w, bias, sums):
+        want = (sums + bias.double()).bfloat16()
+        with torch.cuda.stream(torch.cuda.Stream()):
+            ys = [cb.linear_mxfp4(x, *w, bias) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+            wrong.extend(i for i, y in enumerate(ys) if not same(y, want))
+
+    threads = [threading.Thread(target=work, args=c) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    cb.check_device()
+    assert not wrong
