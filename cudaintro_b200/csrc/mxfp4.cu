@@ -69,13 +69,15 @@ __device__ __forceinline__ void stage512(const T* src, int n, T* dst, int lane) 
   __syncwarp();
 }
 
-// Blocks along the rows of x [R, C].  A warp takes `chunk` words of four scales of a row (a word covers 128 elements): sixteen elements a lane, so a block's largest magnitude is a maximum over two lanes, the codes of a warp
+// Blocks along the rows of x [R, C].  A warp takes STEPS times eight words of four scales of a row (a word covers 128
+// elements): sixteen elements a lane, so a block's largest magnitude is a maximum over two lanes, the codes of a warp
 // leave as 256 contiguous bytes, and eight lanes make a word of scales.  A lane has the loads of UNROLL times 16
 // elements in flight.  The grid also covers the rows that pad the last band of 128, whose scale bytes are zero.
-template <typename T, bool VEC>
+template <typename T, bool VEC, int STEPS>
 __global__ void __launch_bounds__(kMxThreads)
 mx_quantize_rows_kernel(const T* x, uint8_t* q, uint8_t* scale, int64_t R,
-                        int64_t C, int64_t ldx, int words, int chunk, int64_t padded_rows) {
+                        int64_t C, int64_t ldx, int words, int64_t padded_rows) {
+  constexpr int chunk = 8 * STEPS;
   constexpr int UNROLL = sizeof(T) == 4 || !VEC ? 1 : 2;
   __shared__ alignas(16) T stage[VEC ? 1 : kMxThreads / 32][VEC ? 1 : 512];
   const int lane = threadIdx.x & 31;
@@ -222,13 +224,14 @@ mx_quantize_cols_kernel(const T* x, uint8_t* q, uint8_t* scale, int64_t R,
   }
 }
 
-// A warp takes `chunk` elements of a row, a lane 16 bytes of values (eight or four elements) at a time.  VEC (16-byte
-// aligned rows): they are stored as such.  Otherwise the values of 32 x 16 bytes meet in shared memory and leave as words,
-// consecutive lanes consecutive words (stored from the lanes' registers, element by element, rows of 11007 16-bit
+// A warp takes STEPS times 1024 elements of a row, a lane 16 bytes of values (eight or four elements) at a time.  VEC
+// (16-byte aligned rows): they are stored as such.  Otherwise the values of 32 x 16 bytes meet in shared memory and leave
+// as words, consecutive lanes consecutive words (stored from the lanes' registers, element by element, rows of 11007 16-bit
 // values cost 142 us where these take 28).
-template <typename T, bool VEC>
+template <typename T, bool VEC, int STEPS>
 __global__ void __launch_bounds__(kMxThreads)
-mx_dequantize_kernel(const uint8_t* q, const uint8_t* scale, T* x, int64_t rows, int64_t K, int64_t ldx, int words, int chunk) {
+mx_dequantize_kernel(const uint8_t* q, const uint8_t* scale, T* x, int64_t rows, int64_t K, int64_t ldx, int words) {
+  constexpr int chunk = 1024 * STEPS;
   constexpr int N = 16 / int(sizeof(T));  // neighbours a lane takes
   constexpr int UNROLL = 4;
   __shared__ alignas(16) T stage[VEC ? 1 : kMxThreads / 32][VEC ? 1 : 32 * N];
@@ -316,23 +319,26 @@ int launch_in_stream(void (*kernel)(Args...), dim3 grid, cudaStream_t stream, st
   return B200_OK;
 }
 
-// How many of `most` 1024-element steps of a row a warp takes: all of them, or one where that leaves the GPU's warps without
-// work (2048 x 4096 bf16 with four steps a warp: 6.4 us, with one 5.6).
-int steps_per_warp(int64_t rows, int64_t steps, int most) {
-  return rows * ((steps + most - 1) / most) >= 148 * 48 ? most : 1;
+// 1024-element steps of a row that a warp takes: kSteps, or one where kSteps would leave the GPU's warps without work
+// (2048 x 4096 bf16 with four steps a warp: 6.4 us, with one 5.3; back to bf16 7.1 and 5.8 us).  A constant of the
+// kernel: passed as an argument it cost 11008 x 4096 back to bf16 21.0 us where this takes 20.3.
+constexpr int kSteps = 4;
+int steps_per_warp(int64_t rows, int64_t steps) {
+  return rows * ((steps + kSteps - 1) / kSteps) >= 148 * 48 ? kSteps : 1;
 }
 
 template <typename T>
 int quantize_t(const T* x, uint8_t* q, uint8_t* scale, int64_t R, int64_t C, int64_t ldx, int along, cudaStream_t stream) {
   if (along == 0) {
     const int64_t words = (C + 127) / 128, padded = (R + 127) / 128 * 128;
-    const int chunk = 8 * steps_per_warp(R, (words + 7) / 8, 4);
-    const int64_t chunks = (words + chunk - 1) / chunk;
+    const int steps = steps_per_warp(R, (words + 7) / 8);
+    const int64_t chunks = (words + 8 * steps - 1) / (8 * steps);
     if (chunks > 65535) return fail(B200_ERR_TOO_LARGE, "quantize_mxfp4: rows longer than %lld", 65535LL * 1024);
     const dim3 grid(unsigned(padded / (kMxThreads / 32)), unsigned(chunks));
     const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * int64_t(sizeof(T)) % 16 == 0;
-    return launch_in_stream(vec ? mx_quantize_rows_kernel<T, true> : mx_quantize_rows_kernel<T, false>, grid, stream, x, q,
-                            scale, R, C, ldx, int(words), chunk, padded);
+    auto kernel = steps == 1 ? (vec ? mx_quantize_rows_kernel<T, true, 1> : mx_quantize_rows_kernel<T, false, 1>)
+                             : (vec ? mx_quantize_rows_kernel<T, true, kSteps> : mx_quantize_rows_kernel<T, false, kSteps>);
+    return launch_in_stream(kernel, grid, stream, x, q, scale, R, C, ldx, int(words), padded);
   }
   const int64_t words = (R + 127) / 128, padded = (C + 127) / 128 * 128, tall = (words * 128 + kColTileK - 1) / kColTileK;
   const dim3 grid(unsigned(padded / kColTileC), unsigned(tall < 65535 ? tall : 65535));
@@ -344,13 +350,14 @@ int quantize_t(const T* x, uint8_t* q, uint8_t* scale, int64_t R, int64_t C, int
 template <typename T>
 int dequantize_t(const uint8_t* q, const uint8_t* scale, T* x, int64_t rows, int64_t K, int64_t ldx, cudaStream_t stream) {
   const int64_t words = (K + 127) / 128;
-  const int chunk = 1024 * steps_per_warp(rows, (K + 1023) / 1024, 4);
-  const int64_t chunks = (K + chunk - 1) / chunk;
+  const int steps = steps_per_warp(rows, (K + 1023) / 1024);
+  const int64_t chunks = (K + 1024 * steps - 1) / (1024 * steps);
   if (chunks > 65535) return fail(B200_ERR_TOO_LARGE, "dequantize_mxfp4: rows longer than %lld", 65535LL * 1024);
   const dim3 grid(unsigned((rows + kMxThreads / 32 - 1) / (kMxThreads / 32)), unsigned(chunks));
   const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * int64_t(sizeof(T)) % 16 == 0;
-  return launch_in_stream(vec ? mx_dequantize_kernel<T, true> : mx_dequantize_kernel<T, false>, grid, stream, q, scale, x,
-                          rows, K, ldx, int(words), chunk);
+  auto kernel = steps == 1 ? (vec ? mx_dequantize_kernel<T, true, 1> : mx_dequantize_kernel<T, false, 1>)
+                           : (vec ? mx_dequantize_kernel<T, true, kSteps> : mx_dequantize_kernel<T, false, kSteps>);
+  return launch_in_stream(kernel, grid, stream, q, scale, x, rows, K, ldx, int(words));
 }
 
 bool float_dtype(int dtype) { return dtype == B200_F16 || dtype == B200_BF16 || dtype == B200_F32; }
