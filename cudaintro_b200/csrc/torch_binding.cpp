@@ -82,9 +82,10 @@ bool operand(PyObject* q_, PyObject* s_, const at::Tensor** q, const at::Tensor*
   }
   *rows = (*q)->size(0);
   *K = 2 * (*q)->size(1);
-  const at::Tensor& t = **s;
-  if (!*s || t.scalar_type() != at::kByte || t.dim() != 5 || t.size(0) != (*rows + 127) / 128 || t.size(1) != (*K + 127) / 128 ||
-      t.size(2) != 32 || t.size(3) != 4 || t.size(4) != 4 || !t.is_contiguous() || t.device() != (*q)->device()) {
+  const at::Tensor* t = *s;
+  if (!t || t->scalar_type() != at::kByte || t->dim() != 5 || t->size(0) != (*rows + 127) / 128 ||
+      t->size(1) != (*K + 127) / 128 || t->size(2) != 32 || t->size(3) != 4 || t->size(4) != 4 || !t->is_contiguous() ||
+      t->device() != (*q)->device()) {
     refuse("scales are a contiguous uint8 tensor [ceil(rows / 128), ceil(K / 128), 32, 4, 4] beside the packed elements");
     return false;
   }

@@ -364,6 +364,21 @@ def test_wrappers_refuse_what_does_not_belong_together(cb, device):
             pytest.fail(f"call {i} was not refused")
 
 
+def test_what_is_no_tensor_is_refused(cb, device):
+    x = torch.zeros((4, 64), device=device)
+    q, s = cb.quantize_mxfp4(x)
+    for other in (None, 3, [1, 2], "q"):
+        for call in (lambda: cb.quantize_mxfp4(other), lambda: cb.dequantize_mxfp4(other, s), lambda: cb.dequantize_mxfp4(q, other),
+                     lambda: cb.gemm_mxfp4(q, s, q, other), lambda: cb.gemm_mxfp4(q, other, q, s),
+                     lambda: cb.linear_mxfp4(other, q, s), lambda: cb.linear_mxfp4(x, q, other)):
+            with pytest.raises(ValueError):
+                call()
+    for call in (lambda: cb.linear_mxfp4(x, q, s, bias=3), lambda: cb.linear_mxfp4(x, q, s, out=3),
+                 lambda: cb.dequantize_mxfp4(q, s, dtype=3)):
+        with pytest.raises(ValueError):
+            call()
+
+
 # ------------------------------------------------------------------ what the documentation allows besides
 
 
