@@ -108,6 +108,17 @@ bool result(PyObject* given_out, int64_t rows, int64_t cols, at::ScalarType dtyp
   return true;
 }
 
+// A given result that shares memory with an operand would be written while other CTAs still read it.
+bool apart(const at::Tensor& out, std::initializer_list<const at::Tensor*> operands) {
+  const auto begin = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()); };
+  for (const at::Tensor* t : operands)
+    if (t && begin(*t) < begin(out) + out.nbytes() && begin(out) < begin(*t) + t->nbytes()) {
+      refuse("out: must not share memory with an operand");
+      return false;
+    }
+  return true;
+}
+
 // dtype argument: bf16 if not given.
 bool wanted_dtype(PyObject* o, at::ScalarType* dtype) {
   *dtype = at::kBFloat16;
@@ -193,7 +204,7 @@ PyObject* dequantize_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n, PyObj
   if (!wanted_dtype(a[3], &dtype)) return nullptr;
   const at::Device device = q->device();
   at::Tensor out;
-  if (!result(a[4], rows, K, dtype, device, &out)) return nullptr;
+  if (!result(a[4], rows, K, dtype, device, &out) || !apart(out, {q, s})) return nullptr;
   const void *pq = q->const_data_ptr(), *ps = s->const_data_ptr();
   void* po = out.mutable_data_ptr();
   if (!run(device, [&](void* st) { return b200_dequantize_mxfp4(dtype_code(dtype), pq, ps, po, rows, K, 0, st); })) return nullptr;
@@ -213,7 +224,7 @@ PyObject* gemm_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject* k
   at::ScalarType dtype;
   if (!wanted_dtype(v[4], &dtype)) return nullptr;
   at::Tensor out;
-  if (!result(v[5], M, N, dtype, device, &out)) return nullptr;
+  if (!result(v[5], M, N, dtype, device, &out) || !apart(out, {a, sa, b, sb})) return nullptr;
   const void *pa = a->const_data_ptr(), *psa = sa->const_data_ptr(), *pb = b->const_data_ptr(), *psb = sb->const_data_ptr();
   void* po = out.mutable_data_ptr();
   if (!run(device, [&](void* st) { return b200_gemm_mxfp4(dtype_code(dtype), pa, psa, pb, psb, po, M, N, K, 0, st); }))
@@ -238,8 +249,9 @@ PyObject* linear_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject*
   if (in_f <= K - 32 || in_f > K || w->device() != device)
     return refuse("x and w do not fit: their inner dimensions or devices differ");
   const float* bias = nullptr;
+  const at::Tensor* b = nullptr;
   if (given(v[3])) {
-    const at::Tensor* b = tensor(v[3]);
+    b = tensor(v[3]);
     if (!b || b->scalar_type() != at::kFloat || b->dim() != 1 || b->size(0) != out_f || !b->is_contiguous() || b->device() != device)
       return refuse("bias: a contiguous fp32 tensor [out] on the operands' device");
     bias = static_cast<const float*>(b->const_data_ptr());
@@ -247,7 +259,7 @@ PyObject* linear_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject*
   const int relu = v[4] ? PyObject_IsTrue(v[4]) : 0;
   if (relu < 0) return nullptr;
   at::Tensor out, ws;
-  if (!result(v[5], batch, out_f, x->scalar_type(), device, &out)) return nullptr;
+  if (!result(v[5], batch, out_f, x->scalar_type(), device, &out) || !apart(out, {x, w, sw, b})) return nullptr;
   const size_t need = b200_linear_mxfp4_workspace(batch, in_f, out_f);
   void* pws = nullptr;
   if (need) {

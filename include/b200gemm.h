@@ -287,7 +287,8 @@ int b200_linear(int dtype, const void* X, const void* W, const float* bias, void
  *                      ((r / 128) * T + b / 4) * 512 + (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4.
  *                    Bytes of rows and blocks that only fill up a tile must not be 255 (the quantiser
  *                    writes 0).
- * Both arrays are 16-byte aligned, else B200_ERR_UNSUPPORTED. */
+ * Both arrays are 16-byte aligned, else B200_ERR_UNSUPPORTED.  No output of the four operators may share memory
+ * with an input. */
 size_t b200_mxfp4_row_bytes(int64_t K);
 size_t b200_mxfp4_scale_bytes(int64_t rows, int64_t K);
 

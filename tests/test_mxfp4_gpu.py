@@ -379,6 +379,22 @@ def test_what_is_no_tensor_is_refused(cb, device):
             call()
 
 
+def test_results_do_not_share_memory_with_operands(cb, device):
+    x = torch.zeros((256, 256), device=device)
+    q, s = cb.quantize_mxfp4(x)  # q [256, 128] bytes
+    bias = torch.zeros(256 * 256, device=device)
+    room = torch.zeros(2 * 256 * 256, device=device)
+    for call in (lambda: cb.linear_mxfp4(x, q, s, out=x), lambda: cb.linear_mxfp4(x[:1], q, s, out=x[:1]),
+                 lambda: cb.linear_mxfp4(x, q, s, bias[:256], out=bias.view(256, 256)),
+                 lambda: cb.linear_mxfp4(room[:256 * 256].view(256, 256), q, s, out=room[256 * 255:256 * 511].view(256, 256)),
+                 lambda: cb.gemm_mxfp4(q[:32], s[:1], q[:32], s[:1], torch.float16, out=q.view(torch.float16)[:16].view(32, 32)),
+                 lambda: cb.dequantize_mxfp4(q[:1], s[:1], 256, torch.float16, out=q.view(torch.float16)[:4].view(1, 256))):
+        with pytest.raises(ValueError, match="share memory"):
+            call()
+    y = cb.linear_mxfp4(room[:256 * 256].view(256, 256), q, s, out=room[256 * 256:].view(256, 256))  # neighbours
+    assert y.data_ptr() == room.data_ptr() + 4 * 256 * 256 and not y.any()
+
+
 # ------------------------------------------------------------------ what the documentation allows besides
 
 
