@@ -68,7 +68,12 @@ PyObject* refuse(const char* text) {
   return nullptr;
 }
 
-const at::Tensor* tensor(PyObject* o) { return o && THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
+// Null for what is no tensor, and for one whose memory holds the negatives of its values (a view that torch resolves
+// later, such as the imaginary part of a conjugate).
+const at::Tensor* tensor(PyObject* o) {
+  const at::Tensor* t = o && THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
+  return t && !t->is_neg() ? t : nullptr;
+}
 bool given(PyObject* o) { return o && o != Py_None; }
 
 // A packed matrix whose two tensors belong together: rows and K in whole blocks.

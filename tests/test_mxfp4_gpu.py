@@ -379,6 +379,16 @@ def test_what_is_no_tensor_is_refused(cb, device):
             call()
 
 
+def test_values_that_torch_negates_later_are_refused(cb, device):
+    x = torch._neg_view(torch.ones((64, 64), device=device))
+    q, s = cb.quantize_mxfp4(x.resolve_neg())
+    for call in (lambda: cb.quantize_mxfp4(x), lambda: cb.linear_mxfp4(x, q, s), lambda: cb.linear_mxfp4(x.resolve_neg(), q, s, x[0]),
+                 lambda: cb.gemm_mxfp4(q, s, q, s, torch.float32, out=x)):
+        with pytest.raises(ValueError):
+            call()
+    assert same(cb.dequantize_mxfp4(q, s, 64, torch.float32), -torch.ones((64, 64), device=device))
+
+
 def test_results_do_not_share_memory_with_operands(cb, device):
     x = torch.zeros((256, 256), device=device)
     q, s = cb.quantize_mxfp4(x)  # q [256, 128] bytes
