@@ -333,7 +333,7 @@ int quantize_t(const T* x, uint8_t* q, uint8_t* scale, int64_t R, int64_t C, int
     const int64_t words = (C + 127) / 128, padded = (R + 127) / 128 * 128;
     const int steps = steps_per_warp(R, (words + 7) / 8);
     const int64_t chunks = (words + 8 * steps - 1) / (8 * steps);
-    if (chunks > 65535) return fail(B200_ERR_TOO_LARGE, "quantize_mxfp4: rows longer than %lld", 65535LL * 1024);
+    if (chunks > 65535) return fail(B200_ERR_TOO_LARGE, "quantize_mxfp4: rows longer than %lld", 65535LL * 1024 * kSteps);
     const dim3 grid(unsigned(padded / (kMxThreads / 32)), unsigned(chunks));
     const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * int64_t(sizeof(T)) % 16 == 0;
     auto kernel = steps == 1 ? (vec ? mx_quantize_rows_kernel<T, true, 1> : mx_quantize_rows_kernel<T, false, 1>)
@@ -352,7 +352,7 @@ int dequantize_t(const uint8_t* q, const uint8_t* scale, T* x, int64_t rows, int
   const int64_t words = (K + 127) / 128;
   const int steps = steps_per_warp(rows, (K + 1023) / 1024);
   const int64_t chunks = (K + 1024 * steps - 1) / (1024 * steps);
-  if (chunks > 65535) return fail(B200_ERR_TOO_LARGE, "dequantize_mxfp4: rows longer than %lld", 65535LL * 1024);
+  if (chunks > 65535) return fail(B200_ERR_TOO_LARGE, "dequantize_mxfp4: rows longer than %lld", 65535LL * 1024 * kSteps);
   const dim3 grid(unsigned((rows + kMxThreads / 32 - 1) / (kMxThreads / 32)), unsigned(chunks));
   const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * int64_t(sizeof(T)) % 16 == 0;
   auto kernel = steps == 1 ? (vec ? mx_dequantize_kernel<T, true, 1> : mx_dequantize_kernel<T, false, 1>)

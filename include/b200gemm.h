@@ -288,7 +288,8 @@ int b200_linear(int dtype, const void* X, const void* W, const float* bias, void
  *                    Bytes of rows and blocks that only fill up a tile must not be 255 (the quantiser
  *                    writes 0).
  * Both arrays are 16-byte aligned, else B200_ERR_UNSUPPORTED.  No output of the four operators may share memory
- * with an input. */
+ * with an input.  Dimensions go up to 2^30; rows that are quantised along themselves, and those taken back, up to
+ * 2^28 - 4096 elements (B200_ERR_TOO_LARGE). */
 size_t b200_mxfp4_row_bytes(int64_t K);
 size_t b200_mxfp4_scale_bytes(int64_t rows, int64_t K);
 

@@ -78,6 +78,16 @@ def test_refusals(cb):
     assert quant(R=big) == 5 and dequant(K=big, ldx=big) == 5 and gemm(M=big) == 5 and gemm(K=big) == 5 and linear(o=big) == 5
 
 
+def test_rows_that_are_too_long_are_refused_with_their_limit(cb):
+    from cudaintro_b200 import capi
+
+    lib, one, longest = capi.lib, C.c_void_p(64), (1 << 28) - 4096
+    assert lib.b200_quantize_mxfp4(capi.F32, one, one, one, 1, longest + 1, 0, 0, None) == 5
+    assert str(longest).encode() in lib.b200_last_error()
+    assert lib.b200_dequantize_mxfp4(capi.F32, one, one, one, 1, longest + 1, 0, None) == 5
+    assert str(longest).encode() in lib.b200_last_error()
+
+
 def test_no_cpu_fallback(cb):
     if torch.cuda.is_available():
         pytest.skip("this check is for machines without a GPU")
