@@ -8,7 +8,8 @@
 
 The library is a plain C-ABI shared object (see ``include/b200gemm.h``); nothing in it links
 against Python or torch.  Objects are compiled in parallel, one nvcc per source file.  The binding,
-``_torch_binding.so``, is a CPython module of its own (``csrc/torch_binding.cpp``) that links against both.
+``_torch_binding.so``, is a CPython module of its own (``csrc/torch_binding.cpp``) that links against both; where there is
+no torch for it, the library is built alone.
 """
 from __future__ import annotations
 
@@ -57,11 +58,29 @@ BINDING = os.path.join(PKG, "_torch_binding.so")
 BINDING_SOURCE = os.path.join(CSRC, "torch_binding.cpp")
 
 
-def build_binding(force: bool = False) -> str:
-    """Compile the torch binding if it is older than its source or the public header."""
+def binding_obstacle() -> str | None:
+    """What the torch binding lacks on this machine, or None.  The library needs none of it."""
+    try:
+        import torch
+    except ImportError as e:
+        return f"torch cannot be imported ({e})"
+    if torch.version.cuda is None:
+        return "torch was built without CUDA"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "Python.h is not installed"
+    return None
+
+
+def build_binding(force: bool = False) -> str | None:
+    """Compile the torch binding if it is older than its source or the public header.  None, with a note on stderr, where
+    it cannot be compiled for want of torch or Python.h; a compiler that fails is an error."""
     newest = max(_mtime(BINDING_SOURCE), _mtime(os.path.join(ROOT, "include", "b200gemm.h")))
     if not force and _mtime(BINDING) > newest:
         return BINDING
+    obstacle = binding_obstacle()
+    if obstacle:
+        sys.stderr.write(f"the torch binding (the MXFP4 wrappers of the Python package) is not built: {obstacle}\n")
+        return None
     import torch
 
     base = os.path.dirname(torch.__file__)
@@ -79,7 +98,7 @@ def build_binding(force: bool = False) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the library and its torch binding if needed and return the library's path."""
+    """Compile the library, and its torch binding where there is a torch for it, if needed; return the library's path."""
     build_library(force, verbose)
     build_binding(force)
     return LIB
