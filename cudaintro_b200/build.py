@@ -18,6 +18,7 @@ import subprocess
 import sys
 import sysconfig
 from concurrent.futures import ThreadPoolExecutor
+from importlib import metadata
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
@@ -71,11 +72,28 @@ def binding_obstacle() -> str | None:
     return None
 
 
+def binding_target() -> str:
+    """The torch and the Python that a binding compiled now is for."""
+    try:
+        version = metadata.version("torch")
+    except metadata.PackageNotFoundError:
+        version = "unknown"
+    return f"b200 binding for torch {version}, {sysconfig.get_config_var('SOABI')}"
+
+
+def binding_is_current() -> bool:
+    """Whether the binding is newer than its source and the public header, and for this torch and Python (which it carries
+    as text, `built_for`)."""
+    if _mtime(BINDING) <= max(_mtime(BINDING_SOURCE), _mtime(os.path.join(ROOT, "include", "b200gemm.h"))):
+        return False
+    with open(BINDING, "rb") as f:
+        return b"\0" + binding_target().encode() + b"\0" in f.read()
+
+
 def build_binding(force: bool = False) -> str | None:
-    """Compile the torch binding if it is older than its source or the public header.  None, with a note on stderr, where
-    it cannot be compiled for want of torch or Python.h; a compiler that fails is an error."""
-    newest = max(_mtime(BINDING_SOURCE), _mtime(os.path.join(ROOT, "include", "b200gemm.h")))
-    if not force and _mtime(BINDING) > newest:
+    """Compile the torch binding if it is not current.  None, with a note on stderr, where it cannot be compiled for want
+    of torch or Python.h; a compiler that fails is an error."""
+    if not force and binding_is_current():
         return BINDING
     obstacle = binding_obstacle()
     if obstacle:
@@ -86,6 +104,7 @@ def build_binding(force: bool = False) -> str | None:
     base = os.path.dirname(torch.__file__)
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DB200_BUILT_FOR="{binding_target()}"',
            "-I", os.path.join(ROOT, "include"), "-isystem", sysconfig.get_paths()["include"],
            "-isystem", os.path.join(cuda, "include"), "-isystem", os.path.join(base, "include"),
            "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"), BINDING_SOURCE, "-o", BINDING,

@@ -315,4 +315,14 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch_binding", "MXFP4 entry po
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__torch_binding(void) { return PyModule_Create(&g_module); }
+// The torch and the Python this was compiled for; the build looks for this text in the file.
+const char g_built_for[] = "\0" B200_BUILT_FOR;
+
+PyMODINIT_FUNC PyInit__torch_binding(void) {
+  PyObject* module = PyModule_Create(&g_module);
+  if (module && PyModule_AddStringConstant(module, "built_for", g_built_for + 1) < 0) {
+    Py_DECREF(module);
+    return nullptr;
+  }
+  return module;
+}

@@ -70,3 +70,36 @@ def test_a_failing_compiler_is_an_error(build, compiled, monkeypatch):
     monkeypatch.setattr(build.subprocess, "run", lambda cmd, **_: subprocess.CompletedProcess(cmd, 1, "", "no such thing"))
     with pytest.raises(RuntimeError, match="no such thing"):
         build.build()
+
+
+def test_binding_is_compiled_again_for_another_torch_or_python(build, compiled, monkeypatch):
+    """A binding that is newer than its source but was compiled for another torch or Python than those that ask for it."""
+    pytest.importorskip("torch")
+    from importlib import metadata
+
+    build.build()
+    assert len(compiled) == 1
+    with open(build.BINDING, "ab") as f:  # what the compiler makes of the definition on its command line
+        f.write(b"\0" + build.binding_target().encode() + b"\0")
+    assert any(build.binding_target() in word for word in compiled[0])
+    build.build()
+    assert len(compiled) == 1  # up to date
+    version, soabi = metadata.version, build.sysconfig.get_config_var
+    monkeypatch.setattr(build.metadata, "version", lambda name: version(name) + ".post1")
+    build.build()
+    assert len(compiled) == 2 and any(version("torch") + ".post1" in word for word in compiled[1])
+    monkeypatch.setattr(build.metadata, "version", version)
+    monkeypatch.setattr(build.sysconfig, "get_config_var", lambda name: "cpython-399" if name == "SOABI" else soabi(name))
+    build.build()
+    assert len(compiled) == 3 and any("cpython-399" in word for word in compiled[2])
+
+
+def test_built_binding_says_what_it_is_for(build):
+    pytest.importorskip("torch")
+    from cudaintro_b200 import capi
+
+    assert callable(capi.linear_mxfp4)
+    from cudaintro_b200 import _torch_binding
+
+    assert _torch_binding.built_for == build.binding_target()
+    assert build.binding_is_current()
