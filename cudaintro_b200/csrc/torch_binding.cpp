@@ -3,12 +3,14 @@
 // than the same steps take in Python.
 //
 // The module computes nothing and knows no entry points but those of b200gemm.h.  What does not belong together
-// raises ValueError; a failing entry point raises the exception type that capi.py hands over (B200Error).
+// raises ValueError, and so does a tensor whose gradient the call would drop; a failing entry point raises the
+// exception type that capi.py hands over (B200Error).
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -113,6 +115,22 @@ bool result(PyObject* given_out, int64_t rows, int64_t cols, at::ScalarType dtyp
   return true;
 }
 
+// The operators have no derivative, and a result without one would end a gradient in silence: what autograd follows, or
+// would follow into a given result, is refused.
+bool untracked(std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors)
+    if (t && ((c10::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined())) {
+      refuse("a tensor requires a gradient: the MXFP4 operators have none (call them on detached tensors or under torch.no_grad())");
+      return false;
+    }
+  return true;
+}
+
+// A given result was written in place: autograd has to know, should it have kept the values for a backward pass.
+void written(PyObject* given_out, const at::Tensor& out) {
+  if (given(given_out) && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+}
+
 // A given result that shares memory with an operand would be written while other CTAs still read it.
 bool apart(const at::Tensor& out, std::initializer_list<const at::Tensor*> operands) {
   const auto begin = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()); };
@@ -171,6 +189,7 @@ PyObject* quantize_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n, PyObjec
   const int64_t ldx = R == 1 ? C : x->stride(0);
   if ((x->stride(1) != 1 && C != 1) || ldx < C)
     return refuse("x: the elements of a row must be neighbours, and rows must not overlap");
+  if (!untracked({x})) return nullptr;
   long along = 0;
   if (a[1]) {
     along = PyLong_AsLong(a[1]);
@@ -209,10 +228,11 @@ PyObject* dequantize_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n, PyObj
   if (!wanted_dtype(a[3], &dtype)) return nullptr;
   const at::Device device = q->device();
   at::Tensor out;
-  if (!result(a[4], rows, K, dtype, device, &out) || !apart(out, {q, s})) return nullptr;
+  if (!result(a[4], rows, K, dtype, device, &out) || !untracked({&out}) || !apart(out, {q, s})) return nullptr;
   const void *pq = q->const_data_ptr(), *ps = s->const_data_ptr();
   void* po = out.mutable_data_ptr();
   if (!run(device, [&](void* st) { return b200_dequantize_mxfp4(dtype_code(dtype), pq, ps, po, rows, K, 0, st); })) return nullptr;
+  written(a[4], out);
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
@@ -229,11 +249,12 @@ PyObject* gemm_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject* k
   at::ScalarType dtype;
   if (!wanted_dtype(v[4], &dtype)) return nullptr;
   at::Tensor out;
-  if (!result(v[5], M, N, dtype, device, &out) || !apart(out, {a, sa, b, sb})) return nullptr;
+  if (!result(v[5], M, N, dtype, device, &out) || !untracked({&out}) || !apart(out, {a, sa, b, sb})) return nullptr;
   const void *pa = a->const_data_ptr(), *psa = sa->const_data_ptr(), *pb = b->const_data_ptr(), *psb = sb->const_data_ptr();
   void* po = out.mutable_data_ptr();
   if (!run(device, [&](void* st) { return b200_gemm_mxfp4(dtype_code(dtype), pa, psa, pb, psb, po, M, N, K, 0, st); }))
     return nullptr;
+  written(v[5], out);
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
@@ -264,7 +285,8 @@ PyObject* linear_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject*
   const int relu = v[4] ? PyObject_IsTrue(v[4]) : 0;
   if (relu < 0) return nullptr;
   at::Tensor out, ws;
-  if (!result(v[5], batch, out_f, x->scalar_type(), device, &out) || !apart(out, {x, w, sw, b})) return nullptr;
+  if (!result(v[5], batch, out_f, x->scalar_type(), device, &out) || !untracked({x, b, &out}) || !apart(out, {x, w, sw, b}))
+    return nullptr;
   const size_t need = b200_linear_mxfp4_workspace(batch, in_f, out_f);
   void* pws = nullptr;
   if (need) {
@@ -277,6 +299,7 @@ PyObject* linear_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject*
         return b200_linear_mxfp4(code, px, pw, psw, bias, po, batch, in_f, out_f, relu ? B200_LINEAR_RELU : 0, pws, need, st);
       }))
     return nullptr;
+  written(v[5], out);
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
