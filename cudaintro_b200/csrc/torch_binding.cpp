@@ -329,7 +329,8 @@ PyMethodDef g_methods[] = {
     ENTRY(linear_mxfp4,
           "linear_mxfp4(x, w, w_scale, bias=None, relu=False, out=None)\n--\n\n"
           "Fully connected layer on 4-bit weights: act(Q(x) @ W^T + bias), x [batch, in] fp32, fp16 or bf16 quantised\n"
-          "along its rows on the way, (w, w_scale) the quantised [out, in] weights, bias fp32 [out]."),
+          "along its rows on the way, (w, w_scale) the quantised [out, in] weights, bias fp32 [out].  relu is fmaxf(0, .): it\n"
+          "makes 0 of NaN."),
     {"_set_error", set_error, METH_O, "The exception type of failing entry points, called with (status, message)."},
     {nullptr, nullptr, 0, nullptr}};
 

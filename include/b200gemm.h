@@ -320,7 +320,8 @@ int b200_gemm_mxfp4(int out_dtype, const void* A, const void* a_scale, const voi
 /* Fully connected layer on 4-bit weights: Y = act(Q(X) W^T + bias), where Q is b200_quantize_mxfp4 along the
  * rows.  X [batch, in_features] and Y [batch, out_features] are packed row-major matrices of `dtype` (B200_F32,
  * B200_F16 or B200_BF16); W and w_scale a quantised [out_features, in_features] matrix; bias and flags as in
- * b200_linear (the bias is added to the finished fp32 sum).  workspace: device memory for the quantised X,
+ * b200_linear (the bias is added to the finished fp32 sum; B200_LINEAR_RELU is fmaxf(0, .), so an output that is NaN
+ * without it, from a NaN block of W or a NaN or infinity in X, is 0 with it).  workspace: device memory for the quantised X,
  * 16-byte aligned, at least b200_linear_mxfp4_workspace(...) bytes for the same sizes; a call uses it until its
  * work on `stream` is done, so calls that may overlap need one each.  Where that size is 0 (few rows, which
  * the product quantises itself) it may be NULL. */
