@@ -1,10 +1,89 @@
-"""GPU tests of the MXFP4 kernels at sizes that reach each of them, against tests/mxfp4_plain.py."""
+"""GPU tests of the MXFP4 kernels at sizes where each keeps its SMs busy for several rounds, against tests/mxfp4_plain.py:
+CTAs and CTA pairs that work through tiles and rings of shared memory, the layer's tail in every kernel, quantisers whose warps
+take several steps of a row, and scales at both ends of their range.
+
+Bits are compared wherever every partial sum is a number that fp32 holds (as in test_mxfp4_gpu.py)."""
 import pytest
 
-from test_mxfp4_gpu import layer_case, same
+import mxfp4_plain as plain
+from test_mxfp4_gpu import DTYPES, check_quantised, exact_case, generator, layer_case, same
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
+
+
+# M, N, K: five tiles a CTA pair and nine k-blocks each (a ring of five stages), C aligned or not; up to three tiles of a CTA
+PRODUCTS = [(4600, 4360, 2056), (4609, 4355, 2080), (1024, 4096, 2080), (100, 38096, 1544), (100, 38101, 1544), (20000, 40, 1544)]
+
+
+@pytest.mark.parametrize("shape", PRODUCTS)
+def test_product_of_many_tiles_and_many_blocks_is_exact(cb, device, shape):
+    (a, sa), (b, sb), want = exact_case(device, *shape)
+    for dtype in DTYPES:
+        got = cb.gemm_mxfp4(a, sa, b, sb, dtype)
+        cb.check_device()
+        assert same(got, want.to(dtype)), dtype
+
+
+# batch, in, out: CTA pairs with two and five tiles, CTAs with two and three, a split of K, operands that change places
+LAYERS = [(2305, 328, 2184), (2048, 96, 11008), (1024, 96, 4096), (100, 160, 38101), (128, 2816, 264), (100, 2048, 24), (1000, 328, 17),
+          (5000, 64, 32)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layer", LAYERS)
+def test_layers_tail_in_every_kernel(cb, device, layer, dtype):
+    x, (w, sw), bias, sums = layer_case(device, dtype, *layer)
+    for with_bias in (False, True):
+        for relu in (False, True):
+            y = cb.linear_mxfp4(x, w, sw, bias if with_bias else None, relu=relu)
+            cb.check_device()
+            want = sums + bias.double() if with_bias else sums
+            want = want.clamp(min=0) if relu else want
+            assert same(y, want.to(dtype))
+
+
+# rows of more than one group of 4096 elements, enough of them that a warp takes a whole group; 16-byte aligned or not
+BIG = [(8200, 4104, 4104, 0), (7201, 5003, 5003, 0), (7201, 5003, 5008, 1)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("along", [0, 1])
+@pytest.mark.parametrize("rows,cols,pitch,shift", BIG)
+def test_quantisers_of_long_rows_there_and_back(cb, device, rows, cols, pitch, shift, along, dtype):
+    g = generator(device, rows + cols + shift + along)
+    room = torch.randn((rows, pitch), device=device, generator=g)
+    room *= torch.exp2(torch.randint(-6, 7, (rows, 1), device=device, generator=g).float())
+    x = room.to(dtype)[:, shift : shift + cols]
+    q, s = check_quantised(cb, x, along)
+    want = plain.values(*plain.unpack(q, s))[:, : rows if along else cols]
+    for out in DTYPES:
+        q, s = cb.quantize_mxfp4(x, along)  # the way back follows in the stream at once
+        assert same(cb.dequantize_mxfp4(q, s, want.shape[1], out), want.to(out))
+
+
+def test_plain_launches_of_long_rows_give_the_same(cb, device):
+    """Grids that are launched ahead of their predecessor's end, and the same launched plainly."""
+    from cudaintro_b200 import capi
+
+    x = torch.randn((8200, 4104), device=device, generator=generator(device, 6)).bfloat16()
+
+    def everything():
+        out = []
+        for _ in range(3):
+            for along in (0, 1):
+                q, s = cb.quantize_mxfp4(x, along)
+                out += [q, s, cb.dequantize_mxfp4(q, s), cb.gemm_mxfp4(q[:4096], s[:32], q[:200], s[:2])]
+        return out
+
+    first = everything()
+    try:
+        capi.lib.b200_set_dependent_launch(0)
+        second = everything()
+    finally:
+        capi.lib.b200_set_dependent_launch(1)
+    cb.check_device()
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
 
 
 # fused with its quantiser, few rows, exchanged operands, few tiles of a long K, CTAs, CTA pairs
@@ -22,3 +101,19 @@ def test_relu_gives_zero_for_nan(cb, device, layer):
     want = (sums + bias.double()).clamp(min=0)
     want[rows] = 0
     assert same(clipped, want.bfloat16())
+
+
+@pytest.mark.parametrize("shape", [(3, 40, 96), (100, 20, 160), (40, 300, 768), (200, 300, 4096), (2304, 2304, 96)])
+@pytest.mark.parametrize("low_a,low_b", [(-127, 125), (125, -127), (-100, 0), (0, 100), (-60, -60), (-65, -65)])
+def test_scales_at_the_ends_of_their_range(cb, device, shape, low_a, low_b):
+    """Block exponents far below and above 0, up to both ends of the scale byte, where the products and sums are still
+    numbers that fp32 holds: powers of two times the exact case (products 2^(low_a + low_b) .. 2^4 times that)."""
+    M, N, K = shape
+    g = generator(device, M + N + K)
+    high = 2 if max(low_a, low_b) < 126 else 0
+    a, b = plain.random_packed(M, K, low_a, min(low_a + high, 127), g), plain.random_packed(N, K, low_b, min(low_b + high, 127), g)
+    (qa, sa), (qb, sb) = plain.pack(*a), plain.pack(*b)
+    want = plain.values(*a) @ plain.values(*b).t()
+    got = cb.gemm_mxfp4(qa, sa, qb, sb, torch.float32)
+    cb.check_device()
+    assert same(got, want.float())
