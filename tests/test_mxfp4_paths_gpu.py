@@ -117,3 +117,48 @@ def test_scales_at_the_ends_of_their_range(cb, device, shape, low_a, low_b):
     got = cb.gemm_mxfp4(qa, sa, qb, sb, torch.float32)
     cb.check_device()
     assert same(got, want.float())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layer", [(1, 31, 40), (3, 1031, 72), (16, 77, 264), (5, 4099, 136), (16, 11007, 96), (32, 333, 40)])
+def test_small_layers_take_rows_of_any_length_and_views(cb, device, layer, dtype):
+    """Rows that the product quantises itself, aligned to their elements only; x, bias and out begin inside larger tensors,
+    and what lies around the result stays."""
+    batch, in_f, out_f = layer
+    x, (w, sw), bias, sums = layer_case(device, dtype, *layer)
+    if in_f > 7281:  # beyond that fp32 holds the sums only of fewer terms
+        w[:, 2048:] = 0
+        sums = x[:, :4096].double() @ plain.values(*plain.unpack(w, sw))[:, :4096].t()
+    x_room = torch.full((batch * in_f + 3,), float("nan"), dtype=dtype, device=device)
+    bias_room = torch.full((out_f + 1,), float("nan"), device=device)
+    out_room = torch.full((batch * out_f + 2,), 77.0, dtype=dtype, device=device)
+    x_view, bias_view, out = x_room[1:-2].view(batch, in_f), bias_room[1:], out_room[1:-1].view(batch, out_f)
+    x_view.copy_(x)
+    bias_view.copy_(bias)
+    assert cb.linear_mxfp4(x_view, w, sw, bias_view, out=out).data_ptr() == out.data_ptr()
+    cb.check_device()
+    want = (sums + bias.double()).to(dtype)
+    assert same(out, want) and (out_room[[0, -1]] == 77).all()
+    assert same(cb.linear_mxfp4(x, w, sw, bias), want)
+
+
+@pytest.mark.parametrize("layer", [(1, 4096, 1032), (16, 4104, 520), (32, 4096, 136), (3, 96, 18944)])
+def test_a_lost_arrival_in_a_small_layer_is_reported(cb, device, layer):
+    """The kernel that quantises its rows gives up its waits too, and the next call is right."""
+    from cudaintro_b200 import capi
+
+    x, w, bias, sums = layer_case(device, torch.bfloat16, *layer)
+    want = (sums + bias.double()).bfloat16()
+    assert same(cb.linear_mxfp4(x, *w, bias), want)
+    cb.check_device()
+    try:
+        capi._check(capi.lib.b200_test_lose_arrival(0, 50_000_000))
+        cb.linear_mxfp4(x, *w, bias)
+        with pytest.raises(cb.B200Error) as info:
+            cb.check_device()
+        assert info.value.status == 4
+    finally:
+        capi._check(capi.lib.b200_test_lose_arrival(-1, 0))
+    for _ in range(2):
+        assert same(cb.linear_mxfp4(x, *w, bias), want)
+    cb.check_device()
