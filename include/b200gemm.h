@@ -311,7 +311,8 @@ int b200_dequantize_mxfp4(int dtype, const void* q, const void* scale, void* x, 
 
 /* C[m][n] = sum_k A[m][k] * B[n][k] of two packed matrices (both K contiguous, B stored [N, K]) on the tensor
  * cores: exact products, fp32 sums, rounded once to out_dtype (B200_F32, B200_F16, B200_BF16).  A NaN block
- * makes the outputs that take it NaN.  The order of the sums depends on the sizes alone.  ldc = 0 means N; C has no
+ * makes the outputs that take it NaN.  The order of the sums depends on the sizes and on the device's number of SMs,
+ * and on nothing else; b200_linear_mxfp4 may add in another order than this product of the same operands.  ldc = 0 means N; C has no
  * alignment rule beyond its element size.  The tile, store and L2 policies below and above concern the other
  * products; b200_set_dependent_launch, b200_test_lose_arrival and b200_check_device these too. */
 int b200_gemm_mxfp4(int out_dtype, const void* A, const void* a_scale, const void* B, const void* b_scale, void* C,
