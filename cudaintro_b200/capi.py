@@ -239,7 +239,7 @@ def linear(x, w, bias=None, w_layout=ROW_MAJOR_BT, relu=False, bias_first=False,
 
 # ------------------------------------------------------------------ 4-bit (MXFP4)
 # quantize_mxfp4, dequantize_mxfp4, gemm_mxfp4 and linear_mxfp4 are compiled (csrc/torch_binding.cpp): a small product takes
-# the GPU less time than a wrapper written here takes the host (one token through [4096 -> 11008]: 8.4 us on the device,
+# the GPU less time than a wrapper written here takes the host (one token through [4096 -> 11008]: 8.0 us on the device,
 # 10.4 us a call in Python, 5.7 us compiled).  They raise ValueError for arguments that do not belong together or whose
 # gradient would be dropped (there is no derivative), and B200Error for what the library refuses.
 

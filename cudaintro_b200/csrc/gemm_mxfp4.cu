@@ -22,8 +22,8 @@
 // (their commit is waited for), while those of k-block i - 1 keep the tensor pipe busy.
 //
 // Bound: what an SM takes in.  A k-block is 35 KB of operands and scales for 512 clocks of MMAs, and an SM pulls about 84 GB/s
-// out of L2 whatever the clock, 0.42 us a k-block: 8192^3 to bf16 in 187 us in short bursts (5.9 PFLOP/s; without the loads of
-// B 174 us, with half the MMAs 166 us), 220 us under the power cap.  Three, four and five ring stages: 239, 205, 195 us with
+// out of L2 whatever the clock, 0.42 us a k-block: 8192^3 to bf16 in 186 us in short bursts (5.9 PFLOP/s; without the loads of
+// B 174 us, with half the MMAs 166 us), 215 to 224 us under the power cap.  Three, four and five ring stages: 239, 205, 195 us with
 // the clocks read inside; rows per tile-order group 1024 / 2048 / 4096 / 8192 at 8192 x 28672 x 8192, run for seconds, 830 / 799
 // / 769 / 769 us.  Scales written to tensor memory by four warps (tcgen05.st) instead of copied: 437 us.
 //
@@ -535,13 +535,14 @@ constexpr int kSkQuantWarps = 14;
 __host__ __device__ constexpr int sk_threads(int src) { return src == SRC_PACKED ? 256 : 64 + 32 * kSkQuantWarps; }
 constexpr int kSkMaxStages = 12;
 constexpr int kSkMaxPieces = 16;  // pieces of 512 elements in a CTA's range of a token
-// Rows of A the kernel takes.  Against the kernels for 128 x 128 tiles, us: [11008, 4096] weights, 1 row 7.2 / 12.8, 16 rows 9.0 /
-// 12.6, 32 rows 10.7 / 12.6, 64 rows 15.7 / 10.3; [4096, 4096], 32 rows 6.9 / 7.2; [4096, 11008], 64 rows 13.6 / 10.2.
+// (Figures of the few-row and split kernels in this file: bf16, calls in a row in a CUDA graph, weights from HBM.)
+// Rows of A the kernel takes.  Against the kernels for 128 x 128 tiles, us: [11008, 4096] weights, 1 row 7.8 / 12.3, 16 rows 10.1 /
+// 12.2, 32 rows 11.3 / 11.3, 64 rows 16.0 / 10.0; [4096, 4096], 32 rows 7.6 / 7.5; [4096, 11008], 64 rows 14.3 / 10.1.
 constexpr int kSkRows = 32;
 // Rows that the kernel quantises itself, which every tile of features does again, against a quantiser's launch before it.
-// One launch / two, us of a call in a row: 1 row [11008, 4096] 8.7 / 14.4, 16 rows 13.1 / 16.5; 16 rows [4096, 11008] 12.0 /
-// 16.5; 32 rows [4096, 4096] 9.6 / 12.3, [1024, 1024] 7.5 / 10.3; 64 rows [1024, 1024] 11.9 / 8.4; 1 row [28672, 8192], more tiles
-// than SMs, 43.3 / 28.7.  So: up to 16 rows, up to 32 of a limited number of elements, where every tile has an SM.
+// One launch / two, us: 1 row [11008, 4096] 8.0 / 11.2, 16 rows 12.2 / 14.4; 16 rows [4096, 11008] 10.6 / 12.3; 32 rows
+// [4096, 4096] 9.3 / 10.6, [1024, 1024] 7.5 / 9.2; 64 rows [1024, 1024] 10.5 / 7.4; 1 row [28672, 8192], more tiles than SMs,
+// 41.2 / 24.5.  So: up to 16 rows, up to 32 of a limited number of elements, where every tile has an SM.
 constexpr int kSkFusedRows = 16;
 constexpr int64_t kSkFusedElements = 131072, kSkFusedN = 148 * 128;
 constexpr int64_t kSkFusedK = 65536;      // ... and their length: an eighth of it fits in shared memory
@@ -723,9 +724,8 @@ gemm_mx_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   } else if constexpr (SRC != SRC_PACKED) {
     // ------------------------------------------------------------------ tokens -> shared memory
     // A warp takes 512 elements (a piece, two k-blocks) of a token at a time, sixteen a lane, two lanes a block.  The first
-    // piece of all tokens comes first, so that its MMAs can start.  (10 / 14 / 18 warps, us: 1 row [11008, 4096] 8.6 / 8.7 /
-    // 9.1, 16 rows [4096, 11008] 14.5 / 12.3 / 12.4, 32 rows [4096, 4096] 10.4 / 9.6 / 10.0; two pieces at a time in 14: 8.9,
-    // 12.0, 10.0.)
+    // piece of all tokens comes first, so that its MMAs can start.  (10 / 14 / 18 warps, us: 1 row [11008, 4096] 7.8 / 7.9 /
+    // 8.7, 16 rows [4096, 11008] 11.8 / 10.6 / 12.1, 32 rows [4096, 4096] 10.2 / 9.4 / 10.3.)
     const X* x = static_cast<const X*>(p.X);
     const int pieces = (kb_count + 1) / 2;
     const int piece_step = kSkQuantWarps / p.M, m_step = kSkQuantWarps - piece_step * p.M;
@@ -1130,8 +1130,9 @@ int skinny_smem(bool packed, int tokens, int per, int splits, int stages) {
 }
 
 // Cluster size: the largest that asks for at most a quarter more CTAs than there are SMs.  Measured, 1 / 2 / 4 / 8 ranges, us:
-// one row, [11008, 4096] (86 tiles) 9.7 / 8.5 / 13.3 / 14.0; 8 rows, [4096, 4096] (32 tiles) 12.4 / 9.9 / 7.4 / 8.7; 16 rows,
-// [4096, 11008] packed 15.9 / 12.1 / 8.8 / 9.3.
+// one row, [11008, 4096] (86 tiles) 9.3 / 8.0 / 12.1 / 17.3; 8 rows, [4096, 4096] (32 tiles) 9.3 / 7.3 / 6.3 / 7.2; 16 rows,
+// [4096, 11008] packed 15.1 / 11.6 / 9.2 / 10.2.  The shares are uneven: 86 tiles in two ranges are 172 CTAs, so that 24 of 148
+// SMs stream 16 k-blocks where the mean is 9.3; 32 tiles in four are 128 CTAs, and 20 SMs stream nothing.
 SkinnyPlan plan_skinny(const MxGemm& g, bool packed, int sms) {
   SkinnyPlan best;
   const int num_kb = int((g.K + 255) / 256), tokens = int((g.M + 15) / 16) * 16;
@@ -1141,7 +1142,7 @@ SkinnyPlan plan_skinny(const MxGemm& g, bool packed, int sms) {
     const int per = (num_kb + s - 1) / s;
     if ((num_kb + per - 1) / per != s) continue;  // a range would be empty
     // a ring that leaves room for a second CTA on the SM, another cluster's or the next launch's (with all of the SM's
-    // memory one row of the 86-tile layer takes 13.9 us instead of 8.4)
+    // memory one row of the 86-tile layer takes 13.4 us instead of 8.0)
     int stages = per < kSkMaxStages ? per : kSkMaxStages;
     while (stages > 2 && skinny_smem(packed, tokens, per, s, stages) > kSmSharedBytes / 2 - 1024) --stages;
     const int smem = skinny_smem(packed, tokens, per, s, stages);
@@ -1232,11 +1233,11 @@ int device_sms(int* sms) {
   return B200_OK;
 }
 
-// Ranges of K for a product of `tiles` 128 x 128 tiles (1 = do not split).  1 / 2 / 4 / 8 ranges, us: K = 2048, 16 tiles 6.1 /
-// 6.2 / 5.5 / 11.3; K = 4096, 14 tiles 9.2 / 7.3 / 6.1 / 6.6, 32 tiles 9.4 / 7.4 / 7.2 / -, 36 tiles 9.4 / 7.4 / 12.6, 74 tiles 9.6 /
-// 8.0; K = 11008, 14 tiles 19.3 / 11.4 / 8.2 / 7.7, 16 tiles 19.3 / 11.4 / 8.3 / 14.1, 32 tiles 19.6 / 11.7 / 9.3, 74 tiles 20.1 /
-// 13.5.  A cluster has to find its CTAs' SMs inside one group of SMs, so not every SM can be used by clusters of four
-// (seven eighths of them) or eight (three quarters) at once; where a cluster has to wait the time doubles.
+// Ranges of K for a product of `tiles` 128 x 128 tiles (1 = do not split).  1 / 2 / 4 / 8 ranges, us: K = 2048, 16 tiles 6.4 /
+// 6.2 / 5.7 / 11.4; K = 4096, 14 tiles 9.5 / 7.7 / 6.6 / 7.0, 32 tiles 9.5 / 7.5 / 7.3 / 18.8, 36 tiles 9.4 / 7.4 / 12.8 / 19.3, 74
+// tiles 9.8 / 8.6 / 21.0; K = 11008, 14 tiles 19.6 / 12.1 / 8.9 / 8.3, 16 tiles 19.5 / 11.7 / 8.4 / 14.3, 32 tiles 19.7 / 11.9 / 9.6 /
+// 22.4, 74 tiles 19.9 / 13.1 / 27.6.  A cluster has to find its CTAs' SMs inside one group of SMs, so not every SM can be used
+// by clusters of four (seven eighths of them) or eight (three quarters) at once; where a cluster has to wait the time doubles.
 int split_ranges(int64_t tiles, int num_kb, int sms) {
   auto whole = [&](int s) { return ((num_kb + s - 1) / s) * (s - 1) < num_kb; };  // no range is empty
   if (num_kb >= 32 && tiles * 8 * 4 <= int64_t(sms) * 3 && whole(8)) return 8;
@@ -1316,7 +1317,11 @@ int launch_epi(const MxGemm& g, cudaStream_t stream) {
   const int64_t tiles = ((g.M + 127) / 128) * ((g.N + 127) / 128);
   const int splits = split_ranges(tiles, int((g.K + 255) / 256), sms);
   if (splits > 1) return launch_split<EPI>(g, splits, stream);
-  // CTA pairs once they give every pair of SMs a tile.
+  // CTA pairs once they give every pair of SMs a tile.  A k-block takes an SM about as long in either kernel, so what counts is
+  // the rounds of tiles.  Single CTAs / pairs, us, K = 4096 where nothing else is said: 2304 x 2304 22.6 / 16.5, 2048 x 4096 30.0 /
+  // 17.2, 32768 x 128 17.1 / 16.3, 32768 x 64 16.4 / 15.8.  Where fewer pairs have a tile but single CTAs need two rounds, pairs
+  // would be the faster ones too: 1024 x 4096 16.6 / 10.9 (K = 2048: 10.2 / 8.3, K = 11008: 37.1 / 19.2), 256 x 11008 16.4 / 11.5,
+  // 2048 x 2048 with K = 2048 10.3 / 8.2.
   const int64_t pair_tiles = ((g.M + 255) / 256) * ((g.N + 255) / 256);
   if (g.M > 128 && pair_tiles >= sms / 2) return launch_tile<2, 256, EPI>(g, sms, stream);
   return launch_tile<1, 128, EPI>(g, sms, stream);

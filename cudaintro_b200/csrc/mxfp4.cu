@@ -4,8 +4,10 @@
 // exponent and one of mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6).  Declarations and layouts: include/b200gemm.h.
 //
 // Bound: HBM.  A 16-bit element is read once and 17/32 of a byte written (or the reverse).  Measured, inputs rotated
-// through more than L2: 8192 x 8192 bf16 along rows 29.5 us = 5.75 TB/s (0.88 of the measured copy), fp32 53.5 us =
-// 5.7 TB/s, 4096 x 11008 fp16 along columns 21.9 us = 5.2 TB/s, 11008 x 4096 back to bf16 20.3 us = 5.6 TB/s.
+// through more than L2, calls in a row in a CUDA graph: 8192 x 8192 bf16 along rows 29.5 us = 5.75 TB/s (0.88 of the measured
+// copy), fp32 53.3 us = 5.7 TB/s; 4096 x 11008 along columns fp16 21.8 us = 5.25 TB/s, bf16 21.9 us, fp32 32.7 us = 6.2 TB/s; 11008 x
+// 4096 back to bf16 20.6 us = 5.5 TB/s, 8192 x 8192 back to fp32 52.5 us = 5.8 TB/s.  Rows aligned to their element only: 4096 x
+// 11007 fp16 26.5 us along rows and 27.8 back; 4097 x 11007 along columns fp16 41 us, fp32 37.5.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -154,7 +156,7 @@ mx_quantize_cols_kernel(const T* x, uint8_t* q, uint8_t* scale, int64_t R,
       }
     } else if (!VEC && int64_t(blockIdx.x + 1) * kColTileC <= C && r0 + 32 <= R) {
       // inside x, whatever the alignment: no condition between the loads, so that all of them are in flight (with one
-      // each: 156 us for 4097 x 11007, this 41)
+      // each: 156 us for 4097 x 11007 fp16, this 41)
 #pragma unroll
       for (int i = 0; i < 32; ++i, src += ldx) {
         if constexpr (sizeof(T) == 4) {
@@ -300,9 +302,9 @@ mx_dequantize_kernel(const uint8_t* q, const uint8_t* scale, T* x, int64_t rows,
 }
 
 // A grid that fills the GPU is launched so that its CTAs may take their places before the kernel ahead of it in the stream
-// has ended (11008 x 4096 back to bf16, called in a row: 20.3 us, 22.5 plainly).  A smaller one is not: all of it would crowd
-// on the SMs that the kernel ahead leaves first (a layer of 2048 x 4096 -> 11008, whose quantiser has 256 CTAs, called in a
-// row: 57 us, 49 plainly).
+// has ended (11008 x 4096 back to bf16, calls in a row in a CUDA graph: 20.2 us, 20.5 plainly).  A smaller one is not: all of it
+// would crowd on the SMs that the kernel ahead leaves first (a layer of 2048 x 4096 -> 11008, whose quantiser has 256 CTAs: 46.8 us,
+// 44.7 plainly).
 template <typename... Args>
 int launch_in_stream(void (*kernel)(Args...), dim3 grid, cudaStream_t stream, std::decay_t<Args>... args) {
   constexpr int64_t kFull = 148 * 8;  // CTAs of 256 threads that the GPU holds
@@ -320,8 +322,10 @@ int launch_in_stream(void (*kernel)(Args...), dim3 grid, cudaStream_t stream, st
 }
 
 // 1024-element steps of a row that a warp takes: kSteps, or one where kSteps would leave the GPU's warps without work
-// (2048 x 4096 bf16 with four steps a warp: 6.4 us, with one 5.3; back to bf16 7.1 and 5.8 us).  A constant of the
-// kernel: passed as an argument it cost 11008 x 4096 back to bf16 21.0 us where this takes 20.3.
+// (2048 x 4096 with four steps a warp / with one, us: bf16 7.4 / 5.7, fp32 10.9 / 9.1, back to bf16 7.5 / 5.8, to fp32 11.8 / 9.3).
+// Where there are warps enough the two are close, but for fp32 along rows: 8192 x 8192 bf16 29.5 / 29.3, fp32 53.3 / 48.4, back to
+// bf16 29.5 / 29.3, to fp32 52.5 / 51.9; 11008 x 4096 back to bf16 20.7 / 20.6.  A constant of the kernel: as an argument it
+// cost the last of these 3 %.
 constexpr int kSteps = 4;
 int steps_per_warp(int64_t rows, int64_t steps) {
   return rows * ((steps + kSteps - 1) / kSteps) >= 148 * 48 ? kSteps : 1;
