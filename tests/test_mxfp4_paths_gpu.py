@@ -162,3 +162,33 @@ def test_a_lost_arrival_in_a_small_layer_is_reported(cb, device, layer):
     for _ in range(2):
         assert same(cb.linear_mxfp4(x, *w, bias), want)
     cb.check_device()
+
+
+def test_layers_with_workspaces_in_two_graphs_at_once(cb, device):
+    """Layers whose rows are quantised in a launch of their own, captured twice and replayed at the same time on two
+    streams while eager calls run on a third: every one has a workspace to itself."""
+    shapes = [(300, 1024, 520), (2305, 96, 2184), (40, 8192, 72)]
+    cases = [layer_case(device, torch.bfloat16, *s) for s in shapes]
+    exact = [(sums + bias.double()).bfloat16() if s[1] <= 7281 else None for s, (_, _, bias, sums) in zip(shapes, cases)]
+
+    def step():
+        return [cb.linear_mxfp4(x, *w, bias) for x, w, bias, _ in cases]
+
+    alone = step()
+    torch.cuda.synchronize()
+    assert all(want is None or same(y, want) for y, want in zip(alone, exact))
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            outs.append(step() + step())
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(10):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = step()
+    torch.cuda.synchronize()
+    cb.check_device()
+    for ys in (outs[0][:3], outs[0][3:], outs[1][:3], outs[1][3:], eager):
+        assert all(torch.equal(y, want) for y, want in zip(ys, alone))
